@@ -361,6 +361,74 @@ TTB_API int ttb_sdpa_decode_paged(const void *q, const void *k, const void *v, c
                                   int block_size, int pages_per_user, int head_dim, int mask_users, int mask_heads,
                                   float scale, int is_causal, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Attention inside a sliding window, and of a few rows over a long cache (csrc/attention_window.cu).  The token at
+ * position p sees the keys j <= p with j < sinks or j > p - window: the last `window` positions, its own included, and the
+ * first `sinks` ones ("attention sinks").  out = softmax(scale q k^T) v over the keys seen, f32 inside, probabilities
+ * rounded to `dtype` for the second product, the result rounded once; a row that sees no key is zero.  Keys and values
+ * that no row of the call sees are not read, whatever they hold.  No workspace may be shared by calls that can overlap
+ * on the GPU (two streams, or two captured graphs replayed at the same time).
+ *   ttb_sdpa_window         a prompt, or the chunk of one that starts at position `offset`: query row r is the token at
+ *                           r + offset.  q, out [batch, heads_q, seq_q, head_dim], k, v [batch, heads_kv, seq_kv, head_dim];
+ *                           the *_strides3 are host arrays of element strides {batch, head, seq} (null: dense; head_dim is
+ *                           contiguous).  kv_lens (Int32 [batch], nullable): user b has only its first kv_lens[b] keys; rows
+ *                           behind them see what is left of their window.  bf16, f16, f32; any head_dim up to 256.
+ *                           (::ttnn::transformer::scaled_dot_product_attention with sliding_window_size,
+ *                           operations/transformer/scaled_dot_product_attention.cpp)
+ *   ttb_sdpa_window_decode  one token per user, at position cur_pos[b] (Int32 [batch]), whose key and value are in the cache
+ *                           already.  q, out [1, batch, heads, head_dim]; cache [blocks, kv_heads, block_size, head_dim] read
+ *                           through page_table (Int32 [batch, pages_per_user]; entries clamped into range), or, with
+ *                           page_table null, blocks = batch and pages_per_user = 1, [batch, kv_heads, positions, head_dim].
+ *                           A user whose cur_pos is negative gets a zero row; positions behind the table are not seen.
+ *                           `workspace`: ttb_sdpa_window_decode_workspace_bytes(...), positions = pages_per_user * block_size.
+ *   ttb_sdpa_tree           speculative decoding: `nodes` (1 .. 64) drafted tokens per user behind the cached_lens[b] (Int32
+ *                           [batch]) tokens of its cache.  parents (Int32 [parents_users = 1 or batch, nodes]) names each
+ *                           node's parent, an earlier node, or -1 for a node that follows the cached text directly.  A node
+ *                           sees the cached tokens, its ancestors and itself; its position is cached_lens[b] + its depth.
+ *                           q, out [batch, nodes, heads, head_dim], k_draft, v_draft [batch, nodes, kv_heads, head_dim].
+ *                           draft_lens (Int32 [batch], nullable): only the first draft_lens[b] nodes exist, the other rows of
+ *                           out are left as they were.  window = 0: no window.  A parent that is not an earlier node counts
+ *                           as -1 and is reported by ttb_index_status.  `workspace`: ttb_sdpa_tree_workspace_bytes(...).
+ * The last two take bf16 / f16 with head_dim 32, 64, 128 or 256, any number of query heads per kv head, and 16-byte
+ * aligned tensors.  No reference counterpart for the tree (operations/transformer/
+ * paged_scaled_dot_product_attention_decode.cpp is the single-token form). */
+TTB_API int ttb_sdpa_window(const void *q, const void *k, const void *v, const void *kv_lens, void *out, int dtype, int64_t batch,
+                            int64_t heads_q, int64_t heads_kv, int64_t seq_q, int64_t seq_kv, int64_t head_dim,
+                            const int64_t *q_strides3, const int64_t *k_strides3, const int64_t *v_strides3,
+                            const int64_t *out_strides3, int64_t offset, int64_t window, int64_t sinks, float scale, void *stream);
+TTB_API size_t ttb_sdpa_window_decode_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t positions,
+                                                      int64_t window, int64_t sinks);
+TTB_API int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const void *page_table, const void *cur_pos, void *out,
+                                   int dtype, int batch, int heads, int kv_heads, int blocks, int block_size, int pages_per_user,
+                                   int head_dim, int64_t window, int64_t sinks, float scale, void *workspace, size_t workspace_bytes,
+                                   void *stream);
+TTB_API size_t ttb_sdpa_tree_workspace_bytes(int batch, int nodes, int heads, int kv_heads, int head_dim, int64_t positions);
+TTB_API int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const void *k_cache, const void *v_cache,
+                          const void *page_table, const void *cached_lens, const void *parents, const void *draft_lens, void *out,
+                          int dtype, int batch, int nodes, int heads, int kv_heads, int blocks, int block_size, int pages_per_user,
+                          int head_dim, int parents_users, int64_t window, int64_t sinks, float scale, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Upkeep of paged caches [blocks, heads, block_size, head_dim], all caches of a model in one call (csrc/cache_pages.cu).
+ * host_caches / host_drafts are host arrays of `n_caches` device pointers; `dtype` is any type, the elements are moved.
+ *   ttb_paged_copy_blocks   block pairs[i][1] <- block pairs[i][0] in every cache (pairs Int32 [n_pairs, 2]).  A block may be
+ *                           copied to many places; a pair of negatives is padding.  A destination must not be the source of
+ *                           a pair nor the destination of another.  A pair that breaks this (of several with one
+ *                           destination all but the first) or names a block outside the cache is left out and reported by
+ *                           ttb_index_status.  Forks a sequence (its last, partly filled block), reorders beams, and moves
+ *                           the live blocks behind a pool's new end into its holes.
+ *   ttb_paged_commit_draft  appends the accepted path of a draft tree: row path[b][i] of the draft [users, nodes, heads,
+ *                           head_dim] becomes position cached_lens[b] + i of user b, for i < path_lens[b] (path Int32
+ *                           [users, nodes], cached_lens and path_lens Int32 [users], page_table Int32 [users, pages]).  A row
+ *                           without a place (no block in the table, a node outside the draft) is left out and reported by
+ *                           ttb_index_status.  A block that is written must belong to one user only.
+ * No reference counterpart (operations/kv_cache/paged_update_cache.cpp writes the same caches). */
+TTB_API int ttb_paged_copy_blocks(void *const *host_caches, int n_caches, const void *pairs, int n_pairs, int dtype, int64_t blocks,
+                                  int64_t heads, int64_t block_size, int64_t head_dim, void *stream);
+TTB_API int ttb_paged_commit_draft(void *const *host_caches, const void *const *host_drafts, int n_caches, const void *page_table,
+                                   const void *cached_lens, const void *path, const void *path_lens, int dtype, int64_t users,
+                                   int64_t nodes, int64_t heads, int64_t blocks, int64_t block_size, int64_t pages, int64_t head_dim,
+                                   void *stream);
+
 /* ---- indexing: ::ttnn::gather / scatter / sort / topk / sampling (runtime/lib/ttnn/operations/data_movement/
  * {gather,scatter,sort}.cpp, operations/reduction/{topk,sampling}.cpp; goldens tools/golden/mapping.py:5384-5437,
  * 5624-5640, 5927-5958, 5994-6019).
@@ -390,6 +458,24 @@ TTB_API int ttb_sort(const void *x, void *values, void *indices, int dtype, int 
                      size_t take, int descending, void *workspace, size_t workspace_bytes, void *stream);
 TTB_API int ttb_sampling(const void *values, const void *indices, const void *k, const void *p, const void *temp, void *out,
                          int dtype, int index_dtype, int out_dtype, int rows, int candidates, uint64_t seed, void *stream);
+
+/* One draw per row from whole rows of logits [rows, vocab] (element stride row_stride between rows; bf16, f16 or f32),
+ * with the random numbers given (csrc/sampling.cu).  Per row, all in f32 arrays of [rows] but top_k (Int32), each nullable
+ * but `uniform`:
+ *   temperature  w_i = exp((x_i - max x) / temperature); not positive: the largest logit is taken
+ *   top_k        the k largest logits stay, of equal ones the lower index first (k <= 0 or >= vocab: all)
+ *   top_p        of those, in descending order, the shortest prefix whose weight reaches p of their sum (outside (0, 1): all)
+ *   min_p        of those, the ones with w_i >= min_p (outside (0, 1]: all)
+ *   uniform      in [0, 1): the token is the first index, in the vocabulary's order, at which the running sum of the weights
+ *                that stayed exceeds uniform * their total
+ * out (Int32 [rows]) gets the token and prob (f32 [rows], nullable) its share of the weights that stayed.  -inf and NaN
+ * logits are never taken; a row of nothing else gives -1 and 0.  The same inputs give the same token on every run.
+ * `workspace`: ttb_sample_logits_workspace_bytes(...), not shared by calls that can overlap on the GPU.
+ * ttb_sampling draws among pre-selected candidates with its own generator (operations/reduction/sampling.cpp). */
+TTB_API size_t ttb_sample_logits_workspace_bytes(int64_t rows, int64_t vocab);
+TTB_API int ttb_sample_logits(const void *logits, const void *uniform, const void *temperature, const void *top_k, const void *top_p,
+                              const void *min_p, void *out, void *prob, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                              void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- data movement: ::ttnn::permute / slice / concat / repeat / transpose
  * (runtime/lib/ttnn/operations/data_movement/). One gather kernel covers them: out is dense

@@ -364,6 +364,12 @@ static bool fillIdxDims(IdxDims &d, int rank, int dim, const int64_t *idxShape, 
   return true;
 }
 
+// Address of the current device's flag, for kernels of other files that skip a bad index.
+int indexBadFlag(int **flag) {
+  TTB_CUDA(cudaGetSymbolAddress(reinterpret_cast<void **>(flag), g_indexBad));
+  return TTB_OK;
+}
+
 } // namespace ttb
 
 using namespace ttb;
