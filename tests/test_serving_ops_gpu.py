@@ -355,6 +355,40 @@ def test_sample_settings(kn, dtype, vocab):
     check_samples(kn, logits, u, k=[7] * rows)
 
 
+def test_sample_cuts_deep_in_large_rows(kn):
+    """Borders far below the largest logits, where the row has to be searched again."""
+    gen = torch.Generator().manual_seed(21)
+    vocab = 128000
+    k = [40000, 0, 127999, 60000, 3000, 0, 100000, 0, 2500, 9000, 0, 20000]
+    p = [1.0, 0.99, 1.0, 0.97, 0.999, 0.5, 0.9, 0.9999, 1.0, 0.3, 0.8, 1.0]
+    heat = [1.0, 1.5, 1.0, 3.0, 0.7, 8.0, 1.0, 1.0, 0.2, 100.0, 1.0, 0.6]
+    low = [0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 1e-5, 1e-4]
+    logits = torch.randn(len(k), vocab, generator=gen) * 2.5
+    for dtype in (torch.float32, torch.bfloat16):
+        check_samples(kn, logits.to(dtype), torch.rand(len(k), generator=gen).tolist(), heat, k, p, low)
+
+
+def test_sample_rows_that_mislead_a_sample(kn):
+    """Few distinct values, masks of the type's lowest value, almost everything masked, one logit far above the rest."""
+    gen = torch.Generator().manual_seed(22)
+    vocab = 50001
+    x = torch.randn(10, vocab, generator=gen) * 2.5
+    x[0] = 1.25
+    x[1] = torch.randint(0, 3, (vocab,), generator=gen).float()
+    x[2, torch.randperm(vocab, generator=gen)[:49000]] = torch.finfo(torch.float32).min
+    x[3, torch.randperm(vocab, generator=gen)[:49900]] = float("-inf")
+    x[4, 12345] = 900.0
+    x[5, 777] = 3e38
+    x[6, :] = -1e30
+    x[6, 40000:] = 2.0
+    x[7, torch.randperm(vocab, generator=gen)[:vocab - 1]] = float("-inf")
+    x[8, 30000:] = x[8, 0]
+    x[9, 33333] = float("inf")
+    for heat, k, p, low in ((1.0, 0, 1.0, 0.0), (1.0, 30000, 1.0, 0.0), (0.5, 0, 0.95, 0.0), (2.0, 20000, 0.9, 0.01), (0.01, 50, 0.5, 0.0),
+                            (1.0, 0, 1.0, 0.3), (50.0, 45000, 0.99, 0.0), (float("inf"), 49000, 0.75, 0.0), (1e-30, 9, 0.9, 0.5)):
+        check_samples(kn, x, torch.rand(10, generator=gen).tolist(), [heat] * 10, [k] * 10, [p] * 10, [low] * 10)
+
+
 def test_sample_ties_go_to_the_lower_index(kn):
     logits = torch.zeros(6, 1000)
     logits[1, 500:] = 1.0
