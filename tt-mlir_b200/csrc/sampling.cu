@@ -28,32 +28,43 @@ namespace ttb {
 
 constexpr int SL_THREADS = 512;
 constexpr int SL_WARPS = SL_THREADS / 32;
-constexpr int SL_LIST = 8192;               // entries collected by one pass
+constexpr int SL_KEEP = 23;                 // entries a thread can collect in one pass
+constexpr int SL_LIST = 4096;               // entries that fit: 8 per thread on average, 24 once in 10^6 threads
+constexpr int SL_SHORT = 8192;              // rows up to this length fit whole: 16 entries per thread, and one of the ragged ends
 constexpr int SL_SAMPLE = 4096;
+constexpr int SL_STAGES = 6;                // 16-byte vectors of a thread in flight, and the one at work
 constexpr int SL_BINS = 1024;               // two per thread
 constexpr float SL_FIRST = 2500.0f;         // entries aimed at by the first pass
 constexpr float SL_FLOOR = 60.0f;           // octaves below the largest weight that count
-constexpr float SL_UNIT = 68719476736.0f;   // 2^36 units to the largest weight: SL_LIST of them in two 32-bit halves
+constexpr float SL_UNIT = 68719476736.0f;   // 2^36 units to the largest weight: 2^13 of them fit two 32-bit halves
 constexpr int SL_HALF = 18;                 // ... of 18 bits each, whose sums stay below 2^31
 constexpr int64_t SL_MAX_VOCAB = 1 << 22;
-static_assert(SL_BINS == 2 * SL_THREADS && SL_LIST <= 1 << 13, "bins per thread; the halves' sums fit 32 bits");
+static_assert(SL_BINS == 2 * SL_THREADS && SL_THREADS * SL_KEEP < 1 << 14, "bins per thread; the halves' sums fit 32 bits");
 
 // What one pass found: entries at and above lo and hi, weight at and above lo and another bound, the largest logit.
 struct PassResult {
   double mLo, mFrom;
   unsigned int cLo, cHi;
   float top;
+  bool fits; // no thread collected more than it can keep
 };
 
 struct alignas(16) SampleSmem {
-  float listX[SL_LIST];
+  union {
+    uint4 ring[SL_STAGES][SL_THREADS]; // column t: vectors on their way to thread t
+    struct {                           // between the passes
+      unsigned int count[SL_BINS], massLo[SL_BINS], massHi[SL_BINS];
+    };
+  };
+  float list[SL_KEEP][SL_THREADS]; // column t: what thread t collected
   float sample[SL_SAMPLE];
-  unsigned int count[SL_BINS], massLo[SL_BINS], massHi[SL_BINS];
   double dRed[2][SL_WARPS];
-  unsigned long long uRed[2][SL_WARPS], picked[2];
+  unsigned long long uRed[2][SL_WARPS], picked, rest;
   float fRed[2][SL_WARPS];
-  unsigned int cRed[2][SL_WARPS], listN;
+  unsigned int cRed[2][SL_WARPS];
   int iRed[SL_WARPS], pickBin[2];
+  float few[32];
+  unsigned int fewN, equal;
   // the draw's current run and target
   int from, to, ok;
   double target, total;
@@ -91,75 +102,68 @@ template <typename V> __device__ __forceinline__ V slWarpScan(V v) {
 }
 
 // Weights relative to a reference logit: 2^((x - ref) c).  Difference and product are each rounded once, so a weight 2^-h
-// is off by some h 2^-24 of itself.  Entries that must not weigh come as -inf, which any c > 0 makes 0.
-struct ExpWeight {
+// is off by some h 2^-24 of itself.  Under an infinite temperature every finite logit weighs 1 (c = 0); the weight of
+// +-inf then has no value and is never asked for: entries of -inf fail the comparisons around it, and where the largest
+// logit is +inf only its count matters.
+struct Weigher {
   float ref, c;
+  __device__ __forceinline__ void refer(float to, float heat) {
+    ref = heat < INFINITY ? to : 0.0f;
+    c = fminf(1.4426950408889634f / heat, 1e30f);
+  }
   __device__ __forceinline__ float operator()(float x) const {
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((x - ref) * c));
     return w;
   }
 };
-// Infinities, by definition: logits of at least `from` weigh 1, the others nothing.
-struct FlatWeight {
-  float from; // +inf under a largest logit of +inf, the lowest float under an infinite temperature
-  __device__ __forceinline__ float operator()(float x) const { return x >= from ? 1.0f : 0.0f; }
-};
-struct Weigher {
-  float ref, c;
-  bool flat;
-  __device__ __forceinline__ void refer(float to, float heat) {
-    ref = to;
-    c = fminf(fmaxf(1.4426950408889634f / heat, __int_as_float(1)), 1e30f);
-    flat = to == INFINITY || heat == INFINITY;
-  }
-  // Calls f with the weight function as its argument: the hot loops exist once for each kind.
-  template <typename F> __device__ __forceinline__ void with(F &&f) const {
-    if (flat) f(FlatWeight{ref == INFINITY ? INFINITY : -FLT_MAX});
-    else f(ExpWeight{ref, c});
-  }
-  __device__ __forceinline__ float operator()(float x) const {
-    float w = 0.0f;
-    with([&](auto weight) { w = weight(x); });
-    return w;
-  }
-};
 
-// Calls f(x, slot, index) for the entries lo .. hi - 1 of a row and end() after every group, all 32 lanes together.  A
-// group is up to 4 16-byte vectors per lane; slot numbers the lane's entries in it.  x is -inf for a lane without an
-// entry and for NaN.
-template <typename T, typename F, typename E> __device__ __forceinline__ void slForRange(const T *x, int lo, int hi, F &&f, E &&end) {
-  constexpr int VEC = 16 / sizeof(T), UN = sizeof(T) == 4 ? 4 : 2;
+// Calls f(v) for entries lo .. hi - 1 of a row, a few of them (an array) per lane at a time, all 32 lanes together; an
+// entry that a lane does not have is -inf.  The 16-byte vectors of a range are cut into steps of one vector per lane; this
+// warp takes the steps part, part + parts, ... and, as the last of them, the ragged rest.  Vectors come through a ring in
+// shared memory that each lane fills and reads for itself, which keeps them in flight without registers.
+template <typename T, typename F>
+__device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, int hi, int part, int parts, F &&f) {
+  constexpr int VEC = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   if (lo >= hi) return;
   const int skip = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / static_cast<int>(sizeof(T));
-  const int a = min(lo + skip, hi), nv = (hi - a) / VEC;
-  const uint4 *vec = reinterpret_cast<const uint4 *>(x + a);
-  const int full = nv / (32 * UN) * (32 * UN); // vectors in whole groups
-  for (int v0 = 0; v0 < full; v0 += 32 * UN) {
-    uint4 raw[UN];
-#pragma unroll
-    for (int u = 0; u < UN; ++u) raw[u] = __ldg(vec + v0 + u * 32 + lane);
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const T *e = reinterpret_cast<const T *>(&raw[u]);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f(fmaxf(toF32(e[i]), -INFINITY), u * VEC + i, a + (v0 + u * 32 + lane) * VEC + i);
+  const int a = min(lo + skip, hi), steps = (hi - a) / (32 * VEC);
+  const uint4 *vec = reinterpret_cast<const uint4 *>(x + a) + lane;
+  uint4 *ring = &s->ring[0][threadIdx.x];
+  auto fetch = [&](int step, int stage) {
+    if (step < steps) {
+      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + stage * SL_THREADS));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(vec + step * 32) : "memory");
     }
-    end();
-  }
-  // what is left: the entries in front of the first vector, then fewer than 32 UN vectors and the entries behind them
-  if (lo < a) {
-    f(lo + lane < a ? fmaxf(toF32(x[lo + lane]), -INFINITY) : -INFINITY, 0, lo + lane);
-    end();
-  }
-  for (int i0 = a + full * VEC + lane; i0 - lane < hi; i0 += 32 * 8) {
-    float v[8];
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < hi ? toF32(x[i0 + 32 * u]) : -INFINITY;
+  for (int i = 0; i < SL_STAGES - 1; ++i) fetch(part + i * parts, i);
+  int stage = 0;
+#pragma unroll 1
+  for (int c = part; c < steps; c += parts) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(SL_STAGES - 2) : "memory");
+    const uint4 raw = ring[stage * SL_THREADS];
+    const T *e = reinterpret_cast<const T *>(&raw);
+    float v[VEC];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) f(fmaxf(v[u], -INFINITY), u, i0 + 32 * u);
-    end();
+    for (int i = 0; i < VEC; ++i) v[i] = toF32(e[i]);
+    f(v);
+    // the stage read in the step before this one is free: its values have been used
+    fetch(c + (SL_STAGES - 1) * parts, stage == 0 ? SL_STAGES - 1 : stage - 1);
+    stage = stage == SL_STAGES - 1 ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+  if (part != steps % parts) return;
+  // the entries in front of the first vector and behind the last step: fewer than 8, and than 32 VEC
+#pragma unroll 1
+  for (int i0 = lo < a ? lo - 128 : a + steps * 32 * VEC; i0 < hi; i0 = i0 < lo ? a + steps * 32 * VEC : i0 + 128) {
+    const int from = i0 < lo ? lo : i0, stop = i0 < lo ? a : hi;
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = from + 32 * u + lane < stop ? toF32(x[from + 32 * u + lane]) : -INFINITY;
+    f(v);
   }
 }
 
@@ -181,70 +185,87 @@ __device__ __forceinline__ int slRun(int n, int w) {
   return w >= SL_WARPS ? n : min(n, static_cast<int>((static_cast<int64_t>(n) * w / SL_WARPS) & ~31ll));
 }
 
-// One pass over the row.  Entries in [lo, hi) go to the list (s->listN counts them all, also those that do not fit).
-// s->pass gets the entries and (weights) the weight at and above lo and hi, the weight at and above `from`, the largest
-// logit.
-template <typename T>
-__device__ __forceinline__ void slPass(const T *x, int n, SampleSmem *s, const Weigher &weigh, float lo, float hi, float from, bool weights) {
+__device__ __forceinline__ float slMax3(float a, float b, float c) { // a NaN counts as absent
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// One pass over the row.  Entries in [lo, hi) go to the threads' columns; returns how many this thread found (also those
+// that did not fit).  s->pass gets the entries and (WEIGHTS) the weight at and above lo and hi (FIRST: instead of the
+// latter the weight of everything, hi being +inf) and (FIRST) the largest logit.  Comparisons run at half the rate of
+// products and sums, so a step first asks only whether any of a lane's entries can lie in the interval; few do.
+template <bool FIRST, bool WEIGHTS, typename T>
+__device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s, const Weigher &weigh, float lo, float hi) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) s->listN = 0;
-  __syncthreads();
-  float top = -INFINITY, fLo = 0.0f, fFrom = 0.0f;
+  float top = -INFINITY, fLo = 0.0f, fFrom = 0.0f, farCount = 0.0f; // farCount stays below 2^24
   double mLo = 0.0, mFrom = 0.0;
-  unsigned int cHi = 0, hits = 0;
-  float keep[16];
-  auto collect = [&] { // one allocation for the warp's group
-    if (!__any_sync(0xffffffffu, hits)) return;
-    const unsigned int mine = __popc(hits), run = slWarpScan(mine);
-    unsigned int at = 0;
-    if (lane == 31) at = atomicAdd(&s->listN, run);
-    at = __shfl_sync(0xffffffffu, at, 31) + run - mine;
+  unsigned int mine = 0, steps = 0;
+  const float middle = FIRST ? 0.0f : 0.5f * lo + 0.5f * hi, reach = FIRST ? 0.0f : fmaxf(hi - middle, middle - lo) * 1.000001f;
+  float *column = &s->list[0][threadIdx.x];
+  slForRange(x, s, 0, n, warp, SL_WARPS, [&](auto &v) {
+    constexpr int N = sizeof(v) / sizeof(float);
+    bool near;
+    if (FIRST) {
+      float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (hits & (1u << i)) {
-        if (at < SL_LIST) s->listX[at] = keep[i];
-        ++at;
+      for (int i = 0; i < N; i += 2) m = slMax3(m, v[i], v[i + 1]);
+      top = fmaxf(top, m);
+      near = m >= lo;
+    } else {
+      float m = INFINITY; // a NaN (infinite bounds among them) must not hide an entry: the test below is negated
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = fminf(m, fabsf(v[i] - middle));
+      near = !(m > reach);
+    }
+    if (WEIGHTS) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float w = weigh(v[i]);
+        if (FIRST ? v[i] > -INFINITY : v[i] >= hi) fFrom += w;
       }
     }
-    hits = 0;
-  };
-  auto look = [&](float v, int slot) {
-    top = fmaxf(top, v);
-    const bool above = v >= lo, far = v >= hi;
-    if (far) ++cHi;
-    if (above && !far) hits |= 1u << slot;
-    keep[slot] = v;
-  };
-  const int first = slRun(n, warp), last = slRun(n, warp + 1);
-  if (!weights) {
-    slForRange(x, first, last, [&](float v, int slot, int) { look(v, slot); }, collect);
-  } else {
-    weigh.with([&](auto weight) {
-      slForRange(
-          x, first, last,
-          [&](float v, int slot, int) {
-            const float w = weight(v);
-            if (v >= lo) fLo += w;
-            if (v >= from) fFrom += w;
-            look(v, slot);
-          },
-          [&] {
-            mLo += fLo;
-            mFrom += fFrom;
-            fLo = fFrom = 0.0f;
-            collect();
-          });
-    });
+    if (!FIRST) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (v[i] >= hi) farCount += 1.0f;
+      }
+    }
+    if (__any_sync(0xffffffffu, near)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (v[i] >= lo && v[i] < hi) {
+          if (mine < SL_KEEP) column[mine * SL_THREADS] = v[i];
+          ++mine;
+          if (WEIGHTS) fLo += weigh(v[i]);
+        }
+      }
+    }
+    if (WEIGHTS && (++steps & 3) == 0) { // a few f32 sums at a time
+      mLo += fLo;
+      mFrom += fFrom;
+      fLo = fFrom = 0.0f;
+    }
+  });
+  unsigned int cHi = static_cast<unsigned int>(farCount);
+  mLo += fLo;
+  mFrom += fFrom;
+  if (!FIRST) mLo += mFrom; // at and above lo
+  if (WEIGHTS) {
+    mLo = slWarpSum(mLo);
+    mFrom = slWarpSum(mFrom);
   }
-  mLo = slWarpSum(mLo);
-  mFrom = slWarpSum(mFrom);
   top = slWarpMax(top);
   cHi = slWarpSum(cHi);
+  const unsigned int found = slWarpSum(mine);
+  const bool full = __any_sync(0xffffffffu, mine > SL_KEEP);
   if (lane == 0) {
     s->dRed[0][warp] = mLo;
     s->dRed[1][warp] = mFrom;
     s->cRed[0][warp] = cHi;
+    s->cRed[1][warp] = found;
     s->fRed[0][warp] = top;
+    s->iRed[warp] = full;
   }
   __syncthreads();
   if (warp == 0) {
@@ -252,22 +273,27 @@ __device__ __forceinline__ void slPass(const T *x, int n, SampleSmem *s, const W
     mLo = s->dRed[0][l];
     mFrom = s->dRed[1][l];
     cHi = s->cRed[0][l];
+    unsigned int listed = s->cRed[1][l];
     top = slWarpMax(s->fRed[0][l]);
+    const bool anyFull = __any_sync(0xffffffffu, s->iRed[l] != 0);
 #pragma unroll
     for (int o = SL_WARPS / 2; o > 0; o >>= 1) {
       mLo += __shfl_xor_sync(0xffffffffu, mLo, o);
       mFrom += __shfl_xor_sync(0xffffffffu, mFrom, o);
       cHi += __shfl_xor_sync(0xffffffffu, cHi, o);
+      listed += __shfl_xor_sync(0xffffffffu, listed, o);
     }
     if (lane == 0) {
       s->pass.mLo = mLo;
       s->pass.mFrom = mFrom;
       s->pass.cHi = cHi;
-      s->pass.cLo = cHi + s->listN;
+      s->pass.cLo = cHi + listed;
+      s->pass.fits = !anyFull;
       s->pass.top = top;
     }
   }
   __syncthreads();
+  return mine;
 }
 
 // Smallest and largest of v over the block.
@@ -285,87 +311,124 @@ __device__ __forceinline__ void slSpan(SampleSmem *s, float &a, float &b) {
   __syncthreads();
 }
 
-// The border among the list's entries: the first `rest` entries in descending order, or (byMass) entries as long as
-// the units in front of them are fewer than `rest`.  Leaves s->border, s->ties and s->through, the units of the entries
-// that stay.
-__device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, unsigned int count, bool byMass, unsigned long long rest) {
+// The border among the collected entries, which lie in [least, most] (this thread holds `count`): the first `rest` in
+// descending order, or (byMass) entries as long as the units in front of them are fewer than `rest`.  Leaves s->border,
+// s->ties and (weights) s->through, the units of the entries that stay.
+__device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, unsigned int count, bool byMass, bool weights, unsigned long long rest,
+                                         float least, float most) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float *column = &s->list[0][threadIdx.x];
   auto units = [&](float v) { return __float2ull_rn(weigh(v) * SL_UNIT); };
-  float least = INFINITY, most = -INFINITY;
-  for (unsigned int i = threadIdx.x; i < count; i += SL_THREADS) {
-    least = fminf(least, s->listX[i]);
-    most = fmaxf(most, s->listX[i]);
-  }
-  slSpan(s, least, most);
-  unsigned long long through = 0;
-  while (least < most) {
+  for (bool settled = false; !settled;) {
+#pragma unroll 1
     for (int i = threadIdx.x; i < SL_BINS; i += SL_THREADS) s->count[i] = s->massLo[i] = s->massHi[i] = 0;
+    if (threadIdx.x == 0) s->fewN = 0;
     __syncthreads();
-    // least falls into bin 0 and most into the last one or the one before: every round splits what is left.  A range
-    // that overflows is halved twice first; one so narrow that the step overflows still separates its ends.
+    // A range that overflows is shrunk first; one so narrow that the step overflows still separates its ends.
     const float shrink = most - least < INFINITY ? 1.0f : 0.25f, base = least * shrink, step = (SL_BINS - 1) / (most * shrink - base);
-    auto binOf = [&](float v) { return min(static_cast<int>((v * shrink - base) * step), SL_BINS - 1); };
-    for (unsigned int i = threadIdx.x; i < count; i += SL_THREADS) {
-      const float v = s->listX[i];
+    auto binOf = [&](float v) { return max(0, min(static_cast<int>((v * shrink - base) * step), SL_BINS - 1)); };
+#pragma unroll 1
+    for (unsigned int i = 0; i < count; ++i) {
+      const float v = column[i * SL_THREADS];
       if (v >= least && v <= most) {
         const int bin = binOf(v);
-        const unsigned long long w = units(v);
         atomicAdd(&s->count[bin], 1u);
-        atomicAdd(&s->massLo[bin], static_cast<unsigned int>(w & ((1u << SL_HALF) - 1u)));
-        atomicAdd(&s->massHi[bin], static_cast<unsigned int>(w >> SL_HALF));
+        if (byMass) {
+          const unsigned long long w = units(v);
+          atomicAdd(&s->massLo[bin], static_cast<unsigned int>(w & ((1u << SL_HALF) - 1u)));
+          atomicAdd(&s->massHi[bin], static_cast<unsigned int>(w >> SL_HALF));
+        }
       }
     }
     __syncthreads();
     // descending bins: thread t holds bins SL_BINS - 1 - 2t and the one below
     const int b0 = SL_BINS - 1 - 2 * static_cast<int>(threadIdx.x), b1 = b0 - 1;
     auto massOf = [&](int bin) { return (static_cast<unsigned long long>(s->massHi[bin]) << SL_HALF) + s->massLo[bin]; };
-    const unsigned long long m0 = massOf(b0), m1 = massOf(b1);
-    const unsigned long long v0 = byMass ? m0 : s->count[b0], v1 = byMass ? m1 : s->count[b1];
-    unsigned long long all, allMass;
+    const unsigned int c0 = s->count[b0], c1 = s->count[b1];
+    const unsigned long long v0 = byMass ? massOf(b0) : c0, v1 = byMass ? massOf(b1) : c1;
+    unsigned long long all;
     const unsigned long long before = slScan<unsigned long long>(v0 + v1, s->uRed[0], all);
-    const unsigned long long massBefore = slScan<unsigned long long>(m0 + m1, s->uRed[1], allMass);
-    // the bin in which the limit is reached; rounding may leave it just beyond everything: then the last one
+    // The bin in which the limit is reached; rounding may leave it just beyond everything: then the last one that holds
+    // anything.  Where nothing weighs anything the largest value is the border.
     const unsigned long long want = rest < all ? rest : all;
-    if (before < want && want <= before + v0) {
-      s->pickBin[0] = b0;
-      s->picked[0] = before;
-      s->picked[1] = massBefore;
-    } else if (before + v0 < want && want <= before + v0 + v1) {
-      s->pickBin[0] = b1;
-      s->picked[0] = before + v0;
-      s->picked[1] = massBefore + m0;
-    }
-    if (all == 0 && threadIdx.x == 0) { // nothing weighs anything: the largest value is the border
-      s->pickBin[0] = binOf(most);
-      s->picked[0] = s->picked[1] = 0;
+    const bool at0 = before < want && want <= before + v0, at1 = before + v0 < want && want <= before + v0 + v1;
+    if (at0 || at1 || (all == 0 && threadIdx.x == 0)) {
+      s->pickBin[0] = at0 ? b0 : (at1 ? b1 : -1);
+      s->pickBin[1] = static_cast<int>(at0 ? c0 : (at1 ? c1 : 33u));
+      s->picked = at1 ? before + v0 : before;
     }
     __syncthreads();
-    const int bin = s->pickBin[0];
-    rest = want - s->picked[0];
-    through += s->picked[1];
+    const int bin = s->pickBin[0], inBin = s->pickBin[1];
+    rest = want - s->picked;
     // the bin's own entries; entries of one value share a bin
     float a = INFINITY, b = -INFINITY;
-    for (unsigned int i = threadIdx.x; i < count; i += SL_THREADS) {
-      const float v = s->listX[i];
-      if (v >= least && v <= most && binOf(v) == bin) {
+#pragma unroll 1
+    for (unsigned int i = 0; i < count; ++i) {
+      const float v = column[i * SL_THREADS];
+      if (v >= least && v <= most && (bin < 0 || binOf(v) == bin)) {
         a = fminf(a, v);
         b = fmaxf(b, v);
+        if (inBin <= 32) s->few[atomicAdd(&s->fewN, 1u)] = v;
       }
     }
-    slSpan(s, a, b);
-    least = a;
-    most = b;
+    if (inBin <= 32) { // one lane per entry: what lies in front of it, by value
+      __syncthreads();
+      if (warp == 0) {
+        const bool live = lane < inBin;
+        const float v = live ? s->few[lane] : -INFINITY;
+        const unsigned long long each = byMass ? units(v) : 1ull;
+        unsigned long long inFront = 0;
+        unsigned int equal = 0;
+#pragma unroll 1
+        for (int i = 0; i < inBin; ++i) {
+          const float o = __shfl_sync(0xffffffffu, v, i);
+          const unsigned long long oe = __shfl_sync(0xffffffffu, each, i);
+          inFront += o > v ? oe : 0ull;
+          equal += o == v;
+        }
+        // the smallest value with less than `rest` in front of it is the border (rest >= 1: the largest qualifies)
+        const bool in = live && inFront < rest;
+        const float border = slWarpMin(in ? v : INFINITY);
+        if (in && v == border) { // lanes of one value write the same
+          s->border = border;
+          s->rest = rest - inFront;
+          s->equal = equal;
+        }
+      }
+      settled = true;
+    } else {
+      slSpan(s, a, b);
+      least = a;
+      most = b;
+      if (!(a < b) || bin < 0) { // one value (or, without any weight, the largest one)
+        unsigned int equal = 0, allEqual;
+#pragma unroll 1
+        for (unsigned int i = 0; i < count; ++i) equal += column[i * SL_THREADS] == b;
+        slScan<unsigned int>(equal, s->cRed[0], allEqual);
+        if (threadIdx.x == 0) {
+          s->border = b;
+          s->rest = rest;
+          s->equal = allEqual;
+        }
+        settled = true;
+      }
+    }
+    __syncthreads();
   }
-  unsigned int equal = 0, allEqual;
-  for (unsigned int i = threadIdx.x; i < count; i += SL_THREADS) equal += s->listX[i] == least;
-  slScan<unsigned int>(equal, s->cRed[0], allEqual);
-  if (threadIdx.x == 0) {
-    const unsigned long long each = units(least);
-    unsigned long long keep = byMass ? (each ? (rest + each - 1) / each : allEqual) : rest;
-    keep = keep < 1 ? 1 : (keep > allEqual ? allEqual : keep); // a rounded limit may ask for more than there are
-    s->border = least;
-    s->ties = static_cast<unsigned int>(keep);
-    s->through = through + keep * each;
+  const float border = s->border;
+  const unsigned long long each = units(border), per = byMass ? each : 1ull, equal = s->equal;
+  unsigned long long keep = per ? (s->rest + per - 1) / per : equal, above = 0, through;
+  keep = keep < 1 ? 1 : (keep > equal ? equal : keep); // a rounded limit may ask for more than there are
+  if (weights) {
+#pragma unroll 1
+    for (unsigned int i = 0; i < count; ++i) {
+      const float v = column[i * SL_THREADS];
+      above += v > border ? units(v) : 0ull;
+    }
+    slScan<unsigned long long>(above, s->uRed[0], through);
+    if (threadIdx.x == 0) s->through = through + keep * each;
   }
+  if (threadIdx.x == 0) s->ties = static_cast<unsigned int>(keep);
   __syncthreads();
 }
 
@@ -373,26 +436,18 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
 // (byMass: of its weight) lie above; have <= 0: not known, the sample's estimate is taken.  Leaves s->lo and s->hi;
 // lo >= hi: the sample has nothing in the bracket.  Nothing here decides a result, only how soon it is found: f32
 // throughout.
-__device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, float above, bool byMass, float want, float have, int n, int samples) {
-  float a = INFINITY, b = -INFINITY;
-  for (int i = threadIdx.x; i < samples; i += SL_THREADS) {
-    const float v = s->sample[i];
-    if (v >= below && v < above) {
-      a = fminf(a, v);
-      b = fmaxf(b, v);
-    }
-  }
+__device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, float above, float least, float top, bool byMass, float want, float have, int n, int samples) {
+#pragma unroll 1
   for (int i = threadIdx.x; i < SL_BINS; i += SL_THREADS) s->count[i] = 0;
-  slSpan(s, a, b);
-  if (!(a < b) || !(b - a < INFINITY)) { // none, or one value only, or too far apart for bins
-    if (threadIdx.x == 0) {
-      s->lo = a;
-      s->hi = a < INFINITY && !(a < b) ? nextafterf(a, INFINITY) : a;
-    }
+  __syncthreads();
+  const float a = fmaxf(below, least), b = fminf(above, top); // where samples can be
+  if (!(a < b) || !(b - a < INFINITY)) { // one value only, or too far apart for bins
+    if (threadIdx.x == 0) s->lo = s->hi = a;
     __syncthreads();
     return;
   }
   const float step = (SL_BINS - 1) / (b - a), width = (b - a) / (SL_BINS - 1);
+#pragma unroll 1
   for (int i = threadIdx.x; i < samples; i += SL_THREADS) {
     const float v = s->sample[i];
     if (v >= below && v < above) atomicAdd(&s->count[min(static_cast<int>((v - a) * step + 0.5f), SL_BINS - 1)], 1u);
@@ -407,12 +462,27 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     w1 = exp2f((b1 - (SL_BINS - 1)) * width * c);
   }
   float cAll, mAll, qAll;
-  slScan<float>(c0 + c1, s->fRed[0], cAll);
-  const float m0 = slScan<float>(c0 * w0 + c1 * w1, s->fRed[1], mAll) + c0 * w0, m1 = m0 + c1 * w1;
-  const float q0 = slScan<float>(c0 * w0 * w0 + c1 * w1 * w1, s->fRed[0], qAll) + c0 * w0 * w0, q1 = q0 + c1 * w1 * w1;
+  float m0 = slScan<float>(c0 + c1, s->fRed[0], cAll) + c0, m1 = m0 + c1, q0 = m0, q1 = m1;
+  mAll = qAll = cAll;
+  if (byMass) {
+    m0 = slScan<float>(c0 * w0 + c1 * w1, s->fRed[1], mAll) + c0 * w0;
+    m1 = m0 + c1 * w1;
+    q0 = slScan<float>(c0 * w0 * w0 + c1 * w1 * w1, s->fRed[0], qAll) + c0 * w0 * w0;
+    q1 = q0 + c1 * w1 * w1;
+  }
   const float perSample = static_cast<float>(n) / samples;
+  if (cAll * perSample <= 0.75f * SL_LIST) { // the whole bracket will fit
+    if (threadIdx.x == 0) {
+      s->lo = below;
+      s->hi = above;
+    }
+    __syncthreads();
+    return;
+  }
   const float target = fminf(fmaxf(want / (have > 0.0f ? have : cAll * perSample), 0.0f), 1.0f);
-  // Four standard deviations of the sampled share on both sides, less when that would not fit the list.
+  // Four standard deviations of the sampled share on both sides.  When that would not fit, fewer, which fit with a good
+  // chance of a hit; or, should even two be too many, all four, whose counts then bracket the border closely.
+  const float perMass = 1.0f / mAll;
   float margin = 4.0f, pad = 1.5f / samples;
   for (int round = 0;; ++round) {
     if (threadIdx.x == 0) {
@@ -421,13 +491,13 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     }
     __syncthreads();
     auto spread = [&](float q) {
-      return margin * sqrtf(q * (1.0f - target) * (1.0f - target) + fmaxf(qAll - q, 0.0f) * target * target) / mAll + pad;
+      return margin * __fsqrt_rn(q * (1.0f - target) * (1.0f - target) + fmaxf(qAll - q, 0.0f) * target * target) * perMass + pad;
     };
-    const float f0 = m0 / mAll, f1 = m1 / mAll, d0 = spread(q0), d1 = spread(q1);
+    const float f0 = m0 * perMass, f1 = m1 * perMass, d0 = spread(q0), d1 = spread(q1);
     // highest bin that surely lies at or below the border, lowest bin that surely lies in front of it
-    const int least = f0 >= target + d0 ? b0 : (f1 >= target + d1 ? b1 : -1);
-    const int most = f1 <= target - d1 ? b1 : (f0 <= target - d0 ? b0 : SL_BINS);
-    const int wl = __reduce_max_sync(0xffffffffu, least), wm = __reduce_min_sync(0xffffffffu, most);
+    const int under = f0 >= target + d0 ? b0 : (f1 >= target + d1 ? b1 : -1);
+    const int over = f1 <= target - d1 ? b1 : (f0 <= target - d0 ? b0 : SL_BINS);
+    const int wl = __reduce_max_sync(0xffffffffu, under), wm = __reduce_min_sync(0xffffffffu, over);
     if ((threadIdx.x & 31) == 0) {
       if (wl >= 0) atomicMax(&s->pickBin[0], wl);
       if (wm < SL_BINS) atomicMin(&s->pickBin[1], wm);
@@ -438,7 +508,7 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     if (b0 >= pLo && b0 < pHi) inside += s->count[b0];
     if (b1 >= pLo && b1 < pHi) inside += s->count[b1];
     slScan<unsigned int>(inside, s->cRed[0], sum);
-    if (sum * perSample <= 0.8f * SL_LIST || pHi - pLo <= 1 || round == 6) {
+    if (sum * perSample <= SL_LIST || pHi - pLo <= 1 || round == 3) {
       // bin edges lie half a bin below the bins' middles; open ends reach to the bracket's
       if (threadIdx.x == 0) {
         s->lo = pLo < 0 ? below : fmaxf(below, a + (pLo - 0.5f) * width);
@@ -447,8 +517,7 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
       __syncthreads();
       return;
     }
-    margin *= 0.6f;
-    pad = 0.0f;
+    margin = round < 2 ? margin - 1.0f : 4.0f;
   }
 }
 
@@ -458,7 +527,7 @@ template <typename T>
 __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const Weigher &weigh, float border, unsigned int ties, float low, double u, int32_t *out,
                                     float *prob) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float wBorder = border > -INFINITY ? weigh(border) : 0.0f;
+  const float wBorder = border < INFINITY ? (border > -INFINITY ? weigh(border) : 0.0f) : 1.0f;
   const double wEqual = wBorder >= low ? static_cast<double>(wBorder) : 0.0;
   int from = 0, to = n;
   bool whole = true;
@@ -468,19 +537,21 @@ __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const W
     double sum = 0.0;
     float f = 0.0f;
     unsigned int equal = 0;
-    weigh.with([&](auto weight) {
-      slForRange(
-          x, lo, hi,
-          [&](float v, int, int) {
-            const float w = weight(v);
-            if (v > border && !(w < low)) f += w; // an overflowed weight (inf) must show in the total
-            if (v == border) ++equal;
-          },
-          [&] {
-            sum += f;
-            f = 0.0f;
-          });
+    unsigned int steps = 0;
+    slForRange(x, s, lo, hi, 0, 1, [&](auto &v) {
+      constexpr int N = sizeof(v) / sizeof(float);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float w = weigh(v[i]);
+        if (v[i] > border && !(w < low)) f += w; // an overflowed weight (inf, or NaN) must show in the total
+        if (v[i] == border) ++equal;
+      }
+      if ((++steps & 3) == 0) {
+        sum += f;
+        f = 0.0f;
+      }
     });
+    sum += f;
     sum = slWarpSum(sum);
     equal = slWarpSum(equal);
     if (lane == 0) {
@@ -539,45 +610,6 @@ __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const W
   return true;
 }
 
-// The first of the largest logits.
-template <typename T> __device__ __forceinline__ void slGreedy(const T *x, int n, SampleSmem *s, int32_t *out, float *prob) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float top = -INFINITY;
-  int at = 0x7fffffff;
-  slForRange(x, slRun(n, warp), slRun(n, warp + 1),
-             [&](float v, int, int i) {
-               if (v > top || (v == top && i < at)) { // a range's ragged ends do not come in order
-                 top = v;
-                 at = i;
-               }
-             },
-             [] {});
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
-    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-    if (t2 > top || (t2 == top && a2 < at)) {
-      top = t2;
-      at = a2;
-    }
-  }
-  if (lane == 0) {
-    s->fRed[0][warp] = top;
-    s->iRed[warp] = at;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < SL_WARPS; ++w) {
-      if (s->fRed[0][w] > top) { // later warps hold later indices
-        top = s->fRed[0][w];
-        at = s->iRed[w];
-      }
-    }
-    *out = top > -INFINITY ? at : -1;
-    if (prob) *prob = top > -INFINITY ? 1.0f : 0.0f;
-  }
-}
-
 template <typename T>
 __global__ void __launch_bounds__(SL_THREADS, 2)
     sampleLogitsKernel(const T *__restrict__ logits, const float *__restrict__ uniform, const float *__restrict__ temperature,
@@ -595,20 +627,17 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
   out += row;
   if (prob) prob += row;
   const float heat = temperature ? temperature[row] : 1.0f;
-  if (!(heat > 0.0f)) {
-    slGreedy(x, n, s, out, prob);
-    return;
-  }
+  const bool greedy = !(heat > 0.0f); // the first of the largest logits: only it is a candidate
   const int32_t k = topK ? topK[row] : 0;
   const float p = topP ? topP[row] : 1.0f;
-  const bool cutK = k > 0 && k < n, cutP = p > 0.0f && p < 1.0f;
-  float low = minP && minP[row] > 0.0f && minP[row] <= 1.0f ? minP[row] : 0.0f;
+  const bool cutK = !greedy && k > 0 && k < n, cutP = !greedy && p > 0.0f && p < 1.0f;
+  const float low = !greedy && minP && minP[row] > 0.0f && minP[row] <= 1.0f ? minP[row] : 0.0f;
   const double u = fmin(fmax(static_cast<double>(uniform[row]), 0.0), 1.0); // NaN: 0
 
   // ---- a sample: evenly spaced entries, or all of a short row
   const int samples = min(n, SL_SAMPLE);
   const float stride = static_cast<float>(n) / samples;
-  float sTop = -INFINITY, unused = INFINITY;
+  float sTop = -INFINITY, sLeast = INFINITY; // of the finite ones
 #pragma unroll
   for (int i = 0; i < SL_SAMPLE / SL_THREADS; ++i) {
     const int e = tid + i * SL_THREADS;
@@ -616,10 +645,11 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
       const float v = fmaxf(toF32(x[min(n - 1, static_cast<int>(e * stride))]), -INFINITY);
       s->sample[e] = v;
       sTop = fmaxf(sTop, v);
+      if (v > -INFINITY) sLeast = fminf(sLeast, v);
     }
   }
   __syncthreads();
-  slSpan(s, unused, sTop);
+  slSpan(s, sLeast, sTop);
 
   // What stays: entries above `border`, and of those equal to it the first `ties` by index.
   float border = -INFINITY;
@@ -627,26 +657,28 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
   const bool cut = cutK || cutP;
   // Without cuts and a min-p the draw needs no search: weights relative to the sample's largest logit will do, unless
   // that is so small that they overflow.
-  bool exactTop = false, search = cut || low > 0.0f || !(sTop > -INFINITY && sTop < INFINITY);
-  weigh.refer(sTop, heat);
+  bool exactTop = false, search = cut || greedy || low > 0.0f || !(sTop > -INFINITY && sTop < INFINITY);
+  weigh.refer(sTop, greedy ? 1.0f : heat);
   for (;;) {
     if (search) {
       // The list holds the entries in [lo, hi); the border of the cut at work lies in [below, above).
-      bool first = true, again = false, byMass = false;
-      bool ask = cut && n > SL_LIST && sTop > -INFINITY && sTop < INFINITY; // choose an interval first
-      float below = fmaxf(sTop - SL_FLOOR / weigh.c, -FLT_MAX), above = INFINITY, floor = below;
-      float lo = cut ? -FLT_MAX : INFINITY, hi = INFINITY, want = SL_FIRST, have = 0.0f;
+      bool first = true, again = false, byMass = false, infinite = false;
+      bool ask = cut && n > SL_SHORT && sTop > -INFINITY && sTop < INFINITY; // choose an interval first
+      float below = fmaxf(fmaxf(sTop - SL_FLOOR / weigh.c, -FLT_MAX), sLeast), above = INFINITY, floor = below, top = sTop;
+      float lo = cut ? -FLT_MAX : INFINITY, hi = INFINITY, want = SL_FIRST, have = 0.0f, firstLo = INFINITY, borderK = -INFINITY;
+      unsigned int tiesK = 0xffffffffu;
+      double firstMass = 0.0;
       double total = 0.0, atBelow = 0.0, atAbove = 0.0, limit = 0.0, mLo = 0.0, mHi = 0.0;
       int which = cutK ? 0 : 1, round = 0;
       for (bool done = false; !done;) {
         if (ask) {
-          slChoose(s, weigh.c, below, above, byMass, want, have, n, samples);
+          slChoose(s, weigh.c, below, above, sLeast, top, byMass, want, have, n, samples);
           float nLo = s->lo, nHi = s->hi;
           if (first) { // open above, so that it finds the largest logit
             nLo = fminf(nLo, sTop);
             nHi = INFINITY;
-          } else if (!(nLo < nHi) || round >= 6) {
-            // no help from the sample (or it misleads): halve the bracket in the order of the floats
+          } else if (!(nLo < nHi) || (nLo == lo && nHi == hi) || round >= 10) {
+            // no help from the sample, or just what did not fit: halve the bracket in the order of the floats
             auto order = [](float v) {
               const int i = __float_as_int(v);
               return i >= 0 ? static_cast<int64_t>(i) : -static_cast<int64_t>(i & 0x7fffffff);
@@ -662,9 +694,17 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           lo = first ? nLo : fmaxf(nLo, below);
           hi = fminf(nHi, above);
         }
-        slPass(x, n, s, weigh, lo, hi, first ? -FLT_MAX : hi, cutP);
+        unsigned int mine;
+        if (first && !infinite) mine = cutP ? slPass<true, true>(x, n, s, weigh, lo, hi) : slPass<true, false>(x, n, s, weigh, lo, hi);
+        else mine = cutP ? slPass<false, true>(x, n, s, weigh, lo, hi) : slPass<false, false>(x, n, s, weigh, lo, hi);
         const PassResult cur = s->pass;
-        const unsigned int listed = s->listN;
+        if (infinite) { // only the infinite ones weigh anything: both cuts count them
+          border = INFINITY;
+          ties = cur.cHi;
+          if (cutK && static_cast<unsigned int>(k) < ties) ties = static_cast<unsigned int>(k);
+          if (cutP) ties = static_cast<unsigned int>(ceil(static_cast<double>(p) * static_cast<double>(ties)));
+          break;
+        }
         if (first) {
           if (cur.top == -INFINITY) {
             if (tid == 0) {
@@ -675,21 +715,17 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           }
           exactTop = true;
           const double rise = (static_cast<double>(cur.top) - static_cast<double>(sTop)) * weigh.c;
-          weigh.refer(cur.top, heat);
-          if (cur.top == INFINITY) { // only the infinite ones weigh anything: both cuts count them
-            border = FLT_MAX;
-            if (cut) {
-              if (!again) { // how many are there
-                again = true;
-                ask = false;
-                lo = hi = INFINITY;
-                continue;
-              }
-              border = INFINITY;
-              ties = cutK && static_cast<unsigned int>(k) < cur.cHi ? static_cast<unsigned int>(k) : cur.cHi;
-              if (cutP) ties = static_cast<unsigned int>(ceil(static_cast<double>(p) * static_cast<double>(ties)));
-            }
+          weigh.refer(cur.top, greedy ? 1.0f : heat);
+          if (greedy) {
+            border = cur.top;
+            ties = 1;
             break;
+          }
+          if (cur.top == INFINITY) {
+            infinite = true;
+            ask = false;
+            lo = INFINITY;
+            continue;
           }
           if (!cut) break;
           // From here on weights are relative to the true largest logit; the first pass's are rescaled, or taken again
@@ -701,16 +737,20 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
               ask = false;
               continue;
             }
-            rescale = exp2(-rise);
+            rescale = static_cast<double>(exp2f(static_cast<float>(-rise)));
           }
           first = false;
-          floor = fmaxf(cur.top - SL_FLOOR / weigh.c, -FLT_MAX);
+          top = cur.top;
+          floor = fmaxf(top - SL_FLOOR / weigh.c, -FLT_MAX);
           total = cur.mFrom * rescale;
           mHi = 0.0;
           mLo = cur.mLo * rescale;
           byMass = which == 1;
           limit = byMass ? static_cast<double>(p) * total : static_cast<double>(k);
+          firstLo = lo;
+          firstMass = mLo;
           below = floor;
+          above = nextafterf(top, INFINITY);
           atBelow = byMass ? total : 0.0; // entries: not known yet
         } else {
           mHi = cur.mFrom;
@@ -724,9 +764,9 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           const double hiAt = byMass ? mHi : static_cast<double>(cur.cHi), loAt = byMass ? mLo : static_cast<double>(cur.cLo);
           bool found = false;
           if (limit > hiAt && limit <= loAt) {
-            if (listed <= SL_LIST) {
+            if (cur.fits) {
               const double rest = byMass ? ceil((limit - hiAt) * static_cast<double>(SL_UNIT)) : limit - hiAt;
-              slSelect(s, weigh, listed, byMass, static_cast<unsigned long long>(fmax(rest, 1.0)));
+              slSelect(s, weigh, mine, byMass, cutP, static_cast<unsigned long long>(fmax(rest, 1.0)), lo, fminf(hi, top));
               border = s->border;
               ties = s->ties;
               total = mHi + static_cast<double>(s->through) / static_cast<double>(SL_UNIT);
@@ -743,7 +783,7 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
               if (above <= nextafterf(below, INFINITY)) { // one value, more often than the list is long
                 border = below;
                 const double w = static_cast<double>(weigh(below)), each = byMass ? fmax(w, 1e-300) : 1.0;
-                const double keep = fmin(fmax(ceil((limit - hiAt) / each), 1.0), static_cast<double>(listed));
+                const double keep = fmin(fmax(ceil((limit - hiAt) / each), 1.0), static_cast<double>(cur.cLo - cur.cHi));
                 ties = static_cast<unsigned int>(keep);
                 total = mHi + keep * w;
                 found = true;
@@ -765,27 +805,36 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
             found = true;
           }
           if (!found) break; // another interval
+          if (which == 1 && border == borderK) ties = min(ties, tiesK); // rounding must not bring back what top-k dropped
           if (which == 1 || !cutP) {
             done = true;
           } else { // top-p next, among what top-k left
             which = 1;
+            borderK = border;
+            tiesK = ties;
             byMass = true;
             limit = static_cast<double>(p) * total;
-            below = floor;
-            above = INFINITY;
+            below = fmaxf(border, floor);
+            above = nextafterf(top, INFINITY);
             atBelow = total;
             atAbove = 0.0;
             round = 0;
+            if (limit > firstMass) { // what the first pass knows: the sample says little about a few heavy entries
+              above = fminf(above, firstLo);
+              atAbove = firstMass;
+            } else if (firstLo > below) {
+              below = firstLo;
+              atBelow = firstMass;
+            }
           }
         }
         want = static_cast<float>(limit - atAbove);
         have = atBelow > 0.0 ? fmaxf(static_cast<float>(atBelow - atAbove), 1e-30f) : 0.0f;
       }
-      if (cut && weigh.ref < INFINITY && border < floor) {
+      if (cut && border < floor) {
         border = floor;
         ties = 0xffffffffu;
       }
-      low *= weigh(weigh.ref);
     }
     if (slPick(x, n, s, weigh, border, ties, low, u, out, prob) || exactTop) return;
     search = true; // nothing was cut, and the sample's largest logit was too small a reference
