@@ -119,46 +119,53 @@ struct Weigher {
 };
 
 // Calls f(v) for entries lo .. hi - 1 of a row, a few of them (an array) per lane at a time, all 32 lanes together; an
-// entry that a lane does not have is -inf.  The 16-byte vectors of a range are cut into steps of one vector per lane; this
-// warp takes the steps part, part + parts, ... and, as the last of them, the ragged rest.  Vectors come through a ring in
+// entry that a lane does not have is -inf.  The 16-byte vectors of a range are cut into steps of 256 entries; this warp
+// takes the steps part, part + parts, ... and, as the last of them, the ragged rest.  Vectors come through a ring in
 // shared memory that each lane fills and reads for itself, which keeps them in flight without registers.
 template <typename T, typename F>
 __device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, int hi, int part, int parts, F &&f) {
-  constexpr int VEC = 16 / sizeof(T);
+  constexpr int VEC = 16 / sizeof(T), PER = 8 / VEC, AHEAD = SL_STAGES / PER - 1; // entries per vector, vectors per step, steps in flight
   const int lane = threadIdx.x & 31;
   if (lo >= hi) return;
   const int skip = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / static_cast<int>(sizeof(T));
-  const int a = min(lo + skip, hi), steps = (hi - a) / (32 * VEC);
+  const int a = min(lo + skip, hi), steps = (hi - a) / 256;
   const uint4 *vec = reinterpret_cast<const uint4 *>(x + a) + lane;
   uint4 *ring = &s->ring[0][threadIdx.x];
   auto fetch = [&](int step, int stage) {
     if (step < steps) {
-      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + stage * SL_THREADS));
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(vec + step * 32) : "memory");
+      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + stage * (PER * SL_THREADS)));
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst + u * static_cast<uint32_t>(SL_THREADS * sizeof(uint4))),
+                     "l"(vec + step * (32 * PER) + u * 32) : "memory");
+      }
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < SL_STAGES - 1; ++i) fetch(part + i * parts, i);
+  for (int i = 0; i < AHEAD; ++i) fetch(part + i * parts, i);
   int stage = 0;
 #pragma unroll 1
   for (int c = part; c < steps; c += parts) {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(SL_STAGES - 2) : "memory");
-    const uint4 raw = ring[stage * SL_THREADS];
-    const T *e = reinterpret_cast<const T *>(&raw);
-    float v[VEC];
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(AHEAD - 1) : "memory");
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = toF32(e[i]);
+    for (int u = 0; u < PER; ++u) {
+      const uint4 raw = ring[(stage * PER + u) * SL_THREADS];
+      const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[u * VEC + i] = toF32(e[i]);
+    }
     f(v);
     // the stage read in the step before this one is free: its values have been used
-    fetch(c + (SL_STAGES - 1) * parts, stage == 0 ? SL_STAGES - 1 : stage - 1);
-    stage = stage == SL_STAGES - 1 ? 0 : stage + 1;
+    fetch(c + AHEAD * parts, stage == 0 ? AHEAD : stage - 1);
+    stage = stage == AHEAD ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
   if (part != steps % parts) return;
-  // the entries in front of the first vector and behind the last step: fewer than 8, and than 32 VEC
+  // the entries in front of the first vector and behind the last step: fewer than 8 and 256
 #pragma unroll 1
-  for (int i0 = lo < a ? lo - 128 : a + steps * 32 * VEC; i0 < hi; i0 = i0 < lo ? a + steps * 32 * VEC : i0 + 128) {
+  for (int i0 = lo < a ? lo - 128 : a + steps * 256; i0 < hi; i0 = i0 < lo ? a + steps * 256 : i0 + 128) {
     const int from = i0 < lo ? lo : i0, stop = i0 < lo ? a : hi;
     float v[4];
 #pragma unroll
