@@ -639,6 +639,9 @@ static int checkCached(int dtype, int batch, int heads, int kv_heads, int blocks
 }
 
 int indexBadFlag(int **flag); // index_ops.cu: the word that ttb_index_status reports
+int sdpaWindowTcgen05Try(const void *q, const void *k, const void *v, const void *lens, void *out, int dtype, int64_t batch, int64_t hq,
+                         int64_t hkv, int64_t sq, int64_t skv, int64_t dim, const int64_t *qs, const int64_t *ks, const int64_t *vs,
+                         const int64_t *os, int offset, int window, int sinks, float scaleLog2, cudaStream_t st);
 
 } // namespace ttb
 
@@ -687,6 +690,9 @@ int ttb_sdpa_window(const void *q, const void *k, const void *v, const void *kv_
   bool vec = dtype != kF32 && windowMmaDim(head_dim) && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out);
   for (int i = 0; i < 3; ++i) vec = vec && qs[i] % 8 == 0 && ks[i] % 8 == 0 && vs[i] % 8 == 0 && os[i] % 8 == 0;
   if (vec) {
+    const int rc = sdpaWindowTcgen05Try(q, k, v, kv_lens, out, dtype, batch, heads_q, heads_kv, seq_q, seq_kv, head_dim, qs, ks, vs, os, p.offset,
+                                        p.window, p.sinks, p.scaleLog2, st);
+    if (rc >= 0) return rc;
     if (dtype == kBF16) return windowMma<__nv_bfloat16>(q, k, v, nullptr, nullptr, out, head_dim, p, st);
     return windowMma<__half>(q, k, v, nullptr, nullptr, out, head_dim, p, st);
   }

@@ -1,0 +1,404 @@
+// Window attention of a prompt on the 5th-generation tensor cores (ttb_sdpa_window for 16-bit operands with head_dim 64
+// or 128; semantics in attention_window.cu).  Part of attention_tcgen05.cu, whose status word it shares.
+//
+// One CTA owns two row tiles A and B of 128 rows; a row is (query, head of the group), Gp heads of a kv head side by
+// side, so that 2 * 128 / Gp neighbouring queries share every key tile.  Packing heads also keeps the union of the rows'
+// windows short: it is window + 256 / Gp - 1 keys long.  Keys come in tiles of 128, made of two runs of 64 each: first
+// the runs that hold the sinks, then the window's from its first key on, whatever its alignment (a TMA row coordinate has
+// none), so that nothing but the last run is loaded in vain.
+//   warp 0      TMA producer: Q once, then K and V tiles through one ring
+//   warp 1      issues tcgen05.mma: S_A = Q_A K^T, S_B = Q_B K^T, O_A += P_A V, O_B += P_B V
+//   warps 2..5  softmax of tile A, one row per thread;  warps 6..9 of tile B
+// While the softmax warps of one tile work, the tensor pipe runs the other tile's two products.  A tile's probabilities
+// overwrite the first half of the columns of the scores they come from and are read from there as the A operand; a
+// score buffer is rewritten only by a product issued after the one that read its probabilities, so the hand-over needs
+// just two barriers per tile and step (scores there; probabilities there).
+//   TMEM: S_A 0..127, S_B 128..255, O_A 256.., O_B 256 + D..
+//   Shared memory: Q_A | Q_B | ring of K / V tiles | barriers.
+// Bound: 128 x 128 exponentials take the special-function unit as long as the two products of that tile take the tensor
+// pipe.
+#pragma once
+
+namespace ttb {
+
+constexpr int AW_THREADS = 320;
+constexpr int AW_KEYS = 128;                         // keys per tile
+constexpr int AW_RUN = 64;                           // keys per run
+template <int D> struct AwShape {
+  static constexpr int TILE = 128 * D * 2;           // bytes of a Q, K or V tile
+  static constexpr int COLS = 128 * 128;             // bytes of its 64-column part
+  static constexpr int RING = D == 128 ? 5 : 8;      // K and V tiles in turn
+  static constexpr int SMEM = (2 + RING) * TILE + 1024 /* alignment slack */ + 256 /* barriers */;
+};
+
+struct AwParams {
+  int heads, kvHeads, G, Gp, Sq, keys;               // keys: extent of k and v that any row can see
+  int offset, window, sinks;
+  int64_t ob, oh, os;                                // element strides of out over batch, head, query
+  const int32_t *lens;
+  int fmt;                                           // 1 bf16, 0 f16
+  float scaleLog2;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(AW_THREADS, 1)
+    sdpaWindowTcgen05Kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                            const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapSinkK,
+                            const __grid_constant__ CUtensorMap mapSinkV, T *__restrict__ out, AwParams p) {
+  using Sh = AwShape<D>;
+  constexpr int R = Sh::RING, TILE = Sh::TILE, COLS = Sh::COLS;
+  extern __shared__ unsigned char smemRaw[];
+  __shared__ uint32_t tmemBaseSlot;
+  __shared__ int abortFlag;
+
+  const uint32_t base = (smemU32(smemRaw) + 1023u) & ~1023u;
+  const uint32_t sQ = base, sRing = base + 2 * TILE, bars = sRing + R * TILE;
+  const uint32_t qFull = bars, full = bars + 8, empty = full + 8 * R, sFull = empty + 8 * R, pReady = sFull + 16, oFull = pReady + 16,
+                 vClean = oFull + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int perTile = 128 / p.Gp, perCta = 2 * perTile; // queries
+  const int groups = p.G / p.Gp, nQ = (p.Sq + perCta - 1) / perCta;
+  const int qBlock = blockIdx.x % nQ, rest = blockIdx.x / nQ;
+  const int sub = rest % groups, kvh = rest / groups % p.kvHeads, b = rest / groups / p.kvHeads;
+  const int q0 = qBlock * perCta, head0 = kvh * p.G + sub * p.Gp;
+  const int tilesM = q0 + perTile < p.Sq ? 2 : 1; // row tiles with a query
+
+  if (threadIdx.x == 0) {
+    abortFlag = 0;
+    mbarInit(qFull, 1);
+    for (int i = 0; i < R; ++i) {
+      mbarInit(full + 8 * i, 1);
+      mbarInit(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbarInit(sFull + 8 * i, 1);
+      mbarInit(pReady + 8 * i, 4);
+      mbarInit(oFull + 8 * i, 1);
+    }
+    mbarInit(vClean, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemU32(&tmemBaseSlot)), "r"(AT_TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmemBase = tmemBaseSlot;
+  pdlLaunchDependents(); // the prologue above touched no global memory
+  pdlWait();
+  volatile int *abortP = &abortFlag;
+
+  // ---- the CTA's keys: sinks 0 .. sinkN - 1, then start .. n - 1; a window that reaches into the sinks starts behind them
+  const int pMin = p.offset + q0, pMax = p.offset + min(q0 + perCta, p.Sq) - 1;
+  const int len = p.lens ? min(max(p.lens[b], 0), p.keys) : p.keys;
+  const int n = min(len, pMax + 1);
+  const int start = min(max(max(pMin - p.window + 1, 0), p.sinks), n), sinkN = min(p.sinks, n);
+  const int sinkRuns = (sinkN + AW_RUN - 1) / AW_RUN, runs = sinkRuns + (n - start + AW_RUN - 1) / AW_RUN;
+  const int tiles = (runs + 1) / 2;
+  // Rows of the last run behind the user's keys hold anything: their values are cleared before the last product.
+  const int lastKey0 = runs > sinkRuns ? start + (runs - sinkRuns - 1) * AW_RUN : (runs - 1) * AW_RUN;
+  const bool clean = p.lens && runs > 0 && lastKey0 + AW_RUN > len;
+
+  if (warp == 0) {
+    if (lane == 0 && tiles > 0) { // without a key nothing is loaded: no copy may outlive the CTA
+      prefetchTensorMap(&mapQ);
+      prefetchTensorMap(&mapK);
+      prefetchTensorMap(&mapV);
+      mbarArriveExpectTx(qFull, tilesM * TILE);
+      for (int m = 0; m < tilesM; ++m) {
+        for (int c = 0; c < D / 64; ++c) tmaLoad4d(sQ + m * TILE + c * COLS, &mapQ, qFull, c * 64, head0, q0 + m * perTile, b);
+      }
+      auto load = [&](int seq, int tile, const CUtensorMap *map, const CUtensorMap *sinkMap) -> bool {
+        const int s = seq % R, ph = (seq / R) & 1;
+        if (!mbarWait(empty + 8 * s, ph ^ 1, abortP, 1)) return false;
+        mbarArriveExpectTx(full + 8 * s, TILE);
+        for (int h = 0; h < 2; ++h) {
+          const int run = 2 * tile + h;
+          // a run behind the last one starts behind the tensor: zeros
+          const bool sink = run < sinkRuns;
+          const int key = sink ? run * AW_RUN : (run < runs ? start + (run - sinkRuns) * AW_RUN : p.keys);
+          for (int c = 0; c < D / 64; ++c)
+            tmaLoad4d(sRing + s * TILE + c * COLS + h * (COLS / 2), sink ? sinkMap : map, full + 8 * s, c * 64, key, kvh, b);
+        }
+        return true;
+      };
+      for (int j = 0; j < tiles; ++j) {
+        if (!load(2 * j, j, &mapK, &mapSinkK) || !load(2 * j + 1, j, &mapV, &mapSinkV)) break;
+      }
+    }
+    __syncwarp();
+    if (clean) {
+      const int seq = 2 * tiles - 1, s = seq % R;
+      const bool ok = __all_sync(0xffffffffu, mbarWait(full + 8 * s, (seq / R) & 1, abortP, 2));
+      if (ok) {
+        const int first = max(0, len - lastKey0), row0 = ((runs - 1) & 1) * AW_RUN;
+        for (int i = lane; i < (AW_RUN - first) * 8 * (D / 64); i += 32) {
+          const int c = i % 8, col = i / 8 % (D / 64), row = row0 + first + i / 8 / (D / 64);
+          const uint32_t at = sRing + s * TILE + col * COLS + row * 128 + c * 16;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+        }
+        fenceProxyAsyncShared();
+        __syncwarp();
+        if (lane == 0) mbarArrive(vClean);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && tiles > 0) {
+      const uint32_t idS = instrDescF16(p.fmt, 128, AW_KEYS, 0, 0), idPV = instrDescF16(p.fmt, 128, D, 0, 1);
+      bool ok = mbarWait(qFull, 0, abortP, 3);
+      auto scores = [&](int m, int j) { // S_m = Q_m K_j^T: steps of 16 along d, both operands K-major
+        const uint32_t kb = sRing + (2 * j % R) * TILE;
+        tcFenceAfter();
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * COLS + (ks & 3) * 32;
+          tcMma(tmemBase + m * AW_KEYS, smemDescSw128(sQ + m * TILE + off, 0, 1024), smemDescSw128(kb + off, 0, 1024), idS, ks > 0);
+        }
+        tcCommit(sFull + 8 * m);
+      };
+      auto values = [&](int m, int j) { // O_m += P_m V_j: steps of 16 keys; P from tensor memory, V MN-major
+        const uint32_t vb = sRing + ((2 * j + 1) % R) * TILE;
+        tcFenceAfter();
+#pragma unroll
+        for (int ks = 0; ks < AW_KEYS / 16; ++ks)
+          tcMmaTmemA(tmemBase + 2 * AW_KEYS + m * D, tmemBase + m * AW_KEYS + ks * 8, smemDescSw128(vb + ks * 2048, COLS, 1024), idPV,
+                     (j | ks) > 0);
+      };
+      for (int j = 0; ok && j <= tiles; ++j) {
+        if (j < tiles) ok = mbarWait(full + 8 * (2 * j % R), (2 * j / R) & 1, abortP, 4);
+        for (int m = 0; ok && m < tilesM; ++m) {
+          if (j > 0) {
+            const int seq = 2 * j - 1;
+            if (m == 0) ok = mbarWait(full + 8 * (seq % R), (seq / R) & 1, abortP, 5);
+            if (ok && m == 0 && j == tiles && clean) ok = mbarWait(vClean, 0, abortP, 6);
+            if (ok) ok = mbarWait(pReady + 8 * m, (j - 1) & 1, abortP, 7);
+            if (!ok) break;
+            values(m, j - 1);
+            if (m == tilesM - 1) tcCommit(empty + 8 * (seq % R));
+            if (j == tiles) tcCommit(oFull + 8 * m);
+          }
+          if (j < tiles) {
+            scores(m, j);
+            if (m == tilesM - 1) tcCommit(empty + 8 * (2 * j % R));
+          }
+        }
+      }
+    }
+  } else if ((warp - 2) >> 2 < tilesM) {
+    const int m = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane; // TMEM lanes are reachable by warp id mod 4
+    const int qi = q0 + m * perTile + row / p.Gp, pos = p.offset + qi;
+    const int tMin = p.offset + q0 + m * perTile, tMax = tMin + perTile - 1; // positions of this row tile
+    const uint32_t laneAddr = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t sAddr = laneAddr + m * AW_KEYS, oAddr = laneAddr + 2 * AW_KEYS + m * D;
+    const float sl2 = p.scaleLog2;
+    // `ref` is the maximum the exponentials are taken against; it follows the true one only when that has grown by more
+    // than a factor 2^8 (probabilities stay below 2^8), so that most tiles leave O alone.
+    float ref = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      if (!__all_sync(0xffffffffu, mbarWait(sFull + 8 * m, j & 1, abortP, 8))) { ok = false; break; }
+      tcFenceAfter();
+      uint32_t sc[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tcLoad32(sAddr + c * 32, sc[c]);
+      // Visible keys of this row in each run, relative to its first key: lo .. hi.
+      int lo[2], hi[2];
+      bool mask = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int run = 2 * j + h;
+        if (run < sinkRuns) {
+          lo[h] = 0;
+          hi[h] = min(pos, sinkN - 1) - run * AW_RUN;
+          mask |= min(tMin, sinkN - 1) < run * AW_RUN + AW_RUN - 1;
+        } else if (run < runs) {
+          const int key0 = start + (run - sinkRuns) * AW_RUN;
+          lo[h] = pos - p.window + 1 - key0;
+          hi[h] = min(pos, n - 1) - key0;
+          mask |= tMax - p.window + 1 > key0 || min(tMin, n - 1) < key0 + AW_RUN - 1;
+        } else {
+          lo[h] = 1;
+          hi[h] = 0;
+          mask = true;
+        }
+      }
+      tcWaitLd();
+      if (mask) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int at = (c & 1) * 32 + i;
+            if (at < lo[c >> 1] || at > hi[c >> 1]) sc[c][i] = 0xff800000u; // -inf
+          }
+      }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], __uint_as_float(sc[c][i + k]), __uint_as_float(sc[c][i + 4 + k]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      float corr = 1.0f;
+      if (ref == -INFINITY) {
+        ref = mx; // nothing was seen so far: O and l are zero
+      } else if ((mx - ref) * sl2 > 8.0f) {
+        corr = fastExp2((ref - mx) * sl2);
+        ref = mx;
+      }
+      if (__any_sync(0xffffffffu, corr != 1.0f)) {
+        // The scores of this tile were issued behind P V of the one before: O is complete.
+        l *= corr;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          tcLoad32(oAddr + c * 32, r);
+          tcWaitLd();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+          tcStore32(oAddr + c * 32, r);
+        }
+      }
+      const float negM = ref == -INFINITY ? 0.0f : -ref * sl2;
+      const uint64_t sl2x2 = pack2(sl2, sl2), negMx2 = pack2(negM, negM);
+      uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int at = c * 64 + 2 * i;
+          float x, y;
+          unpack2(fma2(pack2u(sc[at >> 5][at & 31], sc[at >> 5][(at & 31) + 1]), sl2x2, negMx2), x, y);
+          x = fastExp2(x);
+          y = fastExp2(y);
+          sum[i & 1] = add2(sum[i & 1], pack2(x, y));
+          w[i] = packPair<T>(x, y);
+        }
+        tcStore32(sAddr + c * 32, w);
+      }
+      tcWaitSt();
+      tcFenceBefore();
+      float s0, s1, s2, s3;
+      unpack2(sum[0], s0, s1);
+      unpack2(sum[1], s2, s3);
+      l += (s0 + s1) + (s2 + s3);
+      __syncwarp();
+      if (lane == 0) mbarArrive(pReady + 8 * m);
+    }
+    if (ok && tiles > 0 && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * m, 0, abortP, 9))) ok = false;
+    if (ok) {
+      tcFenceAfter();
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      T *orow = out + b * p.ob + (head0 + row % p.Gp) * p.oh + qi * p.os;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (tiles > 0) {
+          tcLoad32(oAddr + c * 32, r);
+          tcWaitLd();
+        }
+        if (qi < p.Sq) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 v = make_uint4(0, 0, 0, 0); // a row that sees no key (O may never have been written)
+            if (l > 0.0f) {
+              v.x = packPair<T>(__uint_as_float(r[g * 8]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
+              v.y = packPair<T>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
+              v.z = packPair<T>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
+              v.w = packPair<T>(__uint_as_float(r[g * 8 + 6]) * inv, __uint_as_float(r[g * 8 + 7]) * inv);
+            }
+            *reinterpret_cast<uint4 *>(orow + c * 32 + g * 8) = v;
+          }
+        }
+      }
+    }
+  }
+
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == 1) {
+    tcFenceAfter();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmemBase), "r"(AT_TMEM_COLS) : "memory");
+  }
+}
+
+// 16-bit tensor of 4 dimensions (columns first), 128-byte swizzle, box of 64 columns; a dimension of extent 1 takes any
+// stride.  Rows outside a dimension read as zero.
+static bool makeWindowMap(CUtensorMap *map, const void *ptr, int dtype, const int64_t *extents4, const int64_t *strides3, const int *box3) {
+  EncodeTiledFn fn = encodeTiled();
+  if (!fn) return false;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box3[0]), static_cast<cuuint32_t>(box3[1]), static_cast<cuuint32_t>(box3[2])};
+  cuuint32_t steps[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(extents4[i]);
+  for (int i = 0; i < 3; ++i) {
+    if (extents4[i + 1] > 1 && strides3[i] <= 0) return false;
+    strides[i] = strides3[i] > 0 ? static_cast<cuuint64_t>(strides3[i]) * 2 : 256;
+    if (strides[i] >= (1ull << 40)) return false;
+  }
+  const CUtensorMapDataType dt = dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(map, dt, 4, const_cast<void *>(ptr), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+static int launchWindowTcgen05(const CUtensorMap *maps, void *out, const AwParams &p, unsigned grid, cudaStream_t st) {
+  static bool attrSet[64] = {}; // function attributes belong to a device
+  int dev = 0;
+  TTB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attrSet[dev]) {
+    TTB_CUDA(cudaFuncSetAttribute(sdpaWindowTcgen05Kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, AwShape<D>::SMEM));
+    if (dev >= 0 && dev < 64) attrSet[dev] = true;
+  }
+  TTB_CUDA(launchPdl(sdpaWindowTcgen05Kernel<T, D>, dim3(grid), dim3(AW_THREADS), AwShape<D>::SMEM, st, maps[0], maps[1], maps[2], maps[3],
+                     maps[4], static_cast<T *>(out), p));
+  countLaunch();
+  TTB_LAUNCH_CHECK();
+  return TTB_OK;
+}
+
+// Returns -1 when the problem is outside what this kernel takes (the caller then uses another one), otherwise a status.
+int sdpaWindowTcgen05Try(const void *q, const void *k, const void *v, const void *lens, void *out, int dtype, int64_t batch, int64_t hq,
+                         int64_t hkv, int64_t sq, int64_t skv, int64_t dim, const int64_t *qs, const int64_t *ks, const int64_t *vs,
+                         const int64_t *os, int offset, int window, int sinks, float scaleLog2, cudaStream_t st) {
+  if ((dim != 64 && dim != 128) || (dtype != kBF16 && dtype != kF16) || !(scaleLog2 > 0.0f)) return -1;
+  const int64_t seen = std::min<int64_t>(skv, offset + sq); // keys behind the last row are nobody's
+  if (seen < 1) return -1;
+  AwParams p = {};
+  p.heads = static_cast<int>(hq);
+  p.kvHeads = static_cast<int>(hkv);
+  p.G = static_cast<int>(hq / hkv);
+  p.Gp = 1;
+  while (p.G % (2 * p.Gp) == 0 && p.Gp < 16) p.Gp *= 2;
+  p.Sq = static_cast<int>(sq);
+  p.keys = static_cast<int>(seen);
+  p.offset = offset;
+  p.window = window;
+  p.sinks = sinks;
+  p.ob = os[0]; p.oh = os[1]; p.os = os[2];
+  p.lens = static_cast<const int32_t *>(lens);
+  p.fmt = dtype == kBF16 ? 1 : 0;
+  p.scaleLog2 = scaleLog2;
+  const int64_t perCta = 256 / p.Gp, ctas = (sq + perCta - 1) / perCta * (p.G / p.Gp) * hkv * batch;
+  if (ctas > 0x7fffffff) return -1;
+  CUtensorMap maps[5];
+  const int64_t qe[4] = {dim, hq, sq, batch}, qst[3] = {qs[1], qs[2], qs[0]};
+  const int qbox[3] = {p.Gp, 128 / p.Gp, 1}, kbox[3] = {AW_RUN, 1, 1};
+  if (!makeWindowMap(&maps[0], q, dtype, qe, qst, qbox)) return -1;
+  for (int i = 0; i < 4; ++i) {
+    const bool value = i & 1, sink = i >= 2;
+    const int64_t *s = value ? vs : ks;
+    const int64_t ke[4] = {dim, sink ? std::max<int64_t>(1, std::min<int64_t>(sinks, seen)) : seen, hkv, batch}, kst[3] = {s[2], s[1], s[0]};
+    if (!makeWindowMap(&maps[1 + i], value ? v : k, dtype, ke, kst, kbox)) return -1;
+  }
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (dtype == kBF16) return dim == 64 ? launchWindowTcgen05<__nv_bfloat16, 64>(maps, out, p, grid, st) : launchWindowTcgen05<__nv_bfloat16, 128>(maps, out, p, grid, st);
+  return dim == 64 ? launchWindowTcgen05<__half, 64>(maps, out, p, grid, st) : launchWindowTcgen05<__half, 128>(maps, out, p, grid, st);
+}
+
+} // namespace ttb
