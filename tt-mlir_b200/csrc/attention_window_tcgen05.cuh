@@ -8,20 +8,27 @@
 // none), so that nothing but the last run is loaded in vain.
 //   warp 0      TMA producer: Q once, then K and V tiles through one ring
 //   warp 1      issues tcgen05.mma: S_A = Q_A K^T, S_B = Q_B K^T, O_A += P_A V, O_B += P_B V
-//   warps 2..5  softmax of tile A, one row per thread;  warps 6..9 of tile B
+//   warps 4..7  softmax of tile A, one row per thread;  warps 8..11 of tile B.  They take over most of the registers of the
+//               first four warps (setmaxnreg: 56 + 2 x 224 per thread of each warpgroup = 3 x 168 at launch), which keeps a
+//               row's 128 scores in registers without spills.
 // While the softmax warps of one tile work, the tensor pipe runs the other tile's two products.  A tile's probabilities
 // overwrite the first half of the columns of the scores they come from and are read from there as the A operand; a
 // score buffer is rewritten only by a product issued after the one that read its probabilities, so the hand-over needs
 // just two barriers per tile and step (scores there; probabilities there).
 //   TMEM: S_A 0..127, S_B 128..255, O_A 256.., O_B 256 + D..
 //   Shared memory: Q_A | Q_B | ring of K / V tiles | barriers.
-// Bound: 128 x 128 exponentials take the special-function unit as long as the two products of that tile take the tensor
-// pipe.
+// Measured (32 query / 8 kv heads x 16384 tokens, head_dim 128, window 2048, 64 sinks, bf16): 0.62 ms, 0.86 PFLOP/s, 51 %
+// of the measured cuBLAS rate.  With parts switched off: without exponentials, maxima and sums 0.54 ms, without the
+// products 0.46 ms, without either (loads, tensor-memory traffic, barriers) 0.33 ms, without the TMA loads unchanged.  So
+// neither unit is saturated (43 % of the cycles each): a row tile's chain of scores, hand-over, softmax, hand-over, values
+// is what it waits for, and two row tiles (tensor memory holds no more) overlap only part of it.  Tried and slower: two
+// threads per row with their maxima exchanged (1.35 ms, 96 registers per thread spill), exponentials ahead of the maximum
+// (0.76 ms, spills again).
 #pragma once
 
 namespace ttb {
 
-constexpr int AW_THREADS = 320;
+constexpr int AW_THREADS = 384;
 constexpr int AW_KEYS = 128;                         // keys per tile
 constexpr int AW_RUN = 64;                           // keys per run
 template <int D> struct AwShape {
@@ -53,8 +60,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
 
   const uint32_t base = (smemU32(smemRaw) + 1023u) & ~1023u;
   const uint32_t sQ = base, sRing = base + 2 * TILE, bars = sRing + R * TILE;
-  const uint32_t qFull = bars, full = bars + 8, empty = full + 8 * R, sFull = empty + 8 * R, pReady = sFull + 16, oFull = pReady + 16,
-                 vClean = oFull + 16;
+  const uint32_t qFull = bars, full = bars + 8, empty = full + 8 * R, sFull = empty + 8 * R, pReady = sFull + 16 /* [row tile][half] */,
+                 oFull = pReady + 32, vClean = oFull + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int perTile = 128 / p.Gp, perCta = 2 * perTile; // queries
@@ -73,7 +80,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbarInit(sFull + 8 * i, 1);
-      mbarInit(pReady + 8 * i, 4);
+      mbarInit(pReady + 16 * i, 4);
+      mbarInit(pReady + 16 * i + 8, 4);
       mbarInit(oFull + 8 * i, 1);
     }
     mbarInit(vClean, 1);
@@ -102,217 +110,242 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
   const int lastKey0 = runs > sinkRuns ? start + (runs - sinkRuns - 1) * AW_RUN : (runs - 1) * AW_RUN;
   const bool clean = p.lens && runs > 0 && lastKey0 + AW_RUN > len;
 
-  if (warp == 0) {
-    if (lane == 0 && tiles > 0) { // without a key nothing is loaded: no copy may outlive the CTA
-      prefetchTensorMap(&mapQ);
-      prefetchTensorMap(&mapK);
-      prefetchTensorMap(&mapV);
-      mbarArriveExpectTx(qFull, tilesM * TILE);
-      for (int m = 0; m < tilesM; ++m) {
-        for (int c = 0; c < D / 64; ++c) tmaLoad4d(sQ + m * TILE + c * COLS, &mapQ, qFull, c * 64, head0, q0 + m * perTile, b);
-      }
-      auto load = [&](int seq, int tile, const CUtensorMap *map, const CUtensorMap *sinkMap) -> bool {
-        const int s = seq % R, ph = (seq / R) & 1;
-        if (!mbarWait(empty + 8 * s, ph ^ 1, abortP, 1)) return false;
-        mbarArriveExpectTx(full + 8 * s, TILE);
-        for (int h = 0; h < 2; ++h) {
-          const int run = 2 * tile + h;
-          // a run behind the last one starts behind the tensor: zeros
-          const bool sink = run < sinkRuns;
-          const int key = sink ? run * AW_RUN : (run < runs ? start + (run - sinkRuns) * AW_RUN : p.keys);
-          for (int c = 0; c < D / 64; ++c)
-            tmaLoad4d(sRing + s * TILE + c * COLS + h * (COLS / 2), sink ? sinkMap : map, full + 8 * s, c * 64, key, kvh, b);
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      if (lane == 0 && tiles > 0) { // without a key nothing is loaded: no copy may outlive the CTA
+        prefetchTensorMap(&mapQ);
+        prefetchTensorMap(&mapK);
+        prefetchTensorMap(&mapV);
+        mbarArriveExpectTx(qFull, tilesM * TILE);
+        for (int m = 0; m < tilesM; ++m) {
+          for (int c = 0; c < D / 64; ++c) tmaLoad4d(sQ + m * TILE + c * COLS, &mapQ, qFull, c * 64, head0, q0 + m * perTile, b);
         }
-        return true;
-      };
-      for (int j = 0; j < tiles; ++j) {
-        if (!load(2 * j, j, &mapK, &mapSinkK) || !load(2 * j + 1, j, &mapV, &mapSinkV)) break;
-      }
-    }
-    __syncwarp();
-    if (clean) {
-      const int seq = 2 * tiles - 1, s = seq % R;
-      const bool ok = __all_sync(0xffffffffu, mbarWait(full + 8 * s, (seq / R) & 1, abortP, 2));
-      if (ok) {
-        const int first = max(0, len - lastKey0), row0 = ((runs - 1) & 1) * AW_RUN;
-        for (int i = lane; i < (AW_RUN - first) * 8 * (D / 64); i += 32) {
-          const int c = i % 8, col = i / 8 % (D / 64), row = row0 + first + i / 8 / (D / 64);
-          const uint32_t at = sRing + s * TILE + col * COLS + row * 128 + c * 16;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+        auto load = [&](int seq, int tile, const CUtensorMap *map, const CUtensorMap *sinkMap) -> bool {
+          const int s = seq % R, ph = (seq / R) & 1;
+          if (!mbarWait(empty + 8 * s, ph ^ 1, abortP, 1)) return false;
+          mbarArriveExpectTx(full + 8 * s, TILE);
+          for (int h = 0; h < 2; ++h) {
+            const int run = 2 * tile + h;
+            // a run behind the last one starts behind the tensor: zeros
+            const bool sink = run < sinkRuns;
+            const int key = sink ? run * AW_RUN : (run < runs ? start + (run - sinkRuns) * AW_RUN : p.keys);
+            for (int c = 0; c < D / 64; ++c)
+              tmaLoad4d(sRing + s * TILE + c * COLS + h * (COLS / 2), sink ? sinkMap : map, full + 8 * s, c * 64, key, kvh, b);
+          }
+          return true;
+        };
+        for (int j = 0; j < tiles; ++j) {
+          if (!load(2 * j, j, &mapK, &mapSinkK) || !load(2 * j + 1, j, &mapV, &mapSinkV)) break;
         }
-        fenceProxyAsyncShared();
-        __syncwarp();
-        if (lane == 0) mbarArrive(vClean);
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && tiles > 0) {
-      const uint32_t idS = instrDescF16(p.fmt, 128, AW_KEYS, 0, 0), idPV = instrDescF16(p.fmt, 128, D, 0, 1);
-      bool ok = mbarWait(qFull, 0, abortP, 3);
-      auto scores = [&](int m, int j) { // S_m = Q_m K_j^T: steps of 16 along d, both operands K-major
-        const uint32_t kb = sRing + (2 * j % R) * TILE;
-        tcFenceAfter();
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * COLS + (ks & 3) * 32;
-          tcMma(tmemBase + m * AW_KEYS, smemDescSw128(sQ + m * TILE + off, 0, 1024), smemDescSw128(kb + off, 0, 1024), idS, ks > 0);
+      __syncwarp();
+      if (clean) {
+        const int seq = 2 * tiles - 1, s = seq % R;
+        const bool ok = __all_sync(0xffffffffu, mbarWait(full + 8 * s, (seq / R) & 1, abortP, 2));
+        if (ok) {
+          const int first = max(0, len - lastKey0), row0 = ((runs - 1) & 1) * AW_RUN;
+          for (int i = lane; i < (AW_RUN - first) * 8 * (D / 64); i += 32) {
+            const int c = i % 8, col = i / 8 % (D / 64), row = row0 + first + i / 8 / (D / 64);
+            const uint32_t at = sRing + s * TILE + col * COLS + row * 128 + c * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+          }
+          fenceProxyAsyncShared();
+          __syncwarp();
+          if (lane == 0) mbarArrive(vClean);
         }
-        tcCommit(sFull + 8 * m);
-      };
-      auto values = [&](int m, int j) { // O_m += P_m V_j: steps of 16 keys; P from tensor memory, V MN-major
-        const uint32_t vb = sRing + ((2 * j + 1) % R) * TILE;
-        tcFenceAfter();
-#pragma unroll
-        for (int ks = 0; ks < AW_KEYS / 16; ++ks)
-          tcMmaTmemA(tmemBase + 2 * AW_KEYS + m * D, tmemBase + m * AW_KEYS + ks * 8, smemDescSw128(vb + ks * 2048, COLS, 1024), idPV,
-                     (j | ks) > 0);
-      };
-      for (int j = 0; ok && j <= tiles; ++j) {
-        if (j < tiles) ok = mbarWait(full + 8 * (2 * j % R), (2 * j / R) & 1, abortP, 4);
-        for (int m = 0; ok && m < tilesM; ++m) {
+      }
+    } else if (warp == 1) {
+      if (lane == 0 && tiles > 0) {
+        // One thread issues everything, and 32 products per pair of row tiles and key tile leave it 64 cycles each: the
+        // operand descriptors differ only in the address field of their low word, so each costs one addition (computed in
+        // full for every product, the issuing thread took 3300 cycles per key tile and set the pace).
+        constexpr uint32_t IDV = (2u << 29) | (1u << 14) | (1024u >> 4); // high word: 128-byte swizzle, version, 1024 bytes per 8 rows
+        const uint32_t idS = instrDescF16(p.fmt, 128, AW_KEYS, 0, 0), idPV = instrDescF16(p.fmt, 128, D, 0, 1);
+        auto desc = [](uint32_t low) -> uint64_t { return (static_cast<uint64_t>(IDV) << 32) | low; };
+        const uint32_t qLow = sQ >> 4, ringLow = sRing >> 4, apart = static_cast<uint32_t>(COLS >> 4) << 16; // V: distance of its 64-column parts
+        bool ok = mbarWait(qFull, 0, abortP, 3);
+        int slot = 0, phase = 0; // of the next tile in the ring
+        auto advance = [&] {
+          if (++slot == R) {
+            slot = 0;
+            phase ^= 1;
+          }
+        };
+        for (int j = 0; ok && j <= tiles; ++j) {
+          // the ring holds V_{j-1} (from the second round on), then K_j
+          const int vSlot = slot;
           if (j > 0) {
-            const int seq = 2 * j - 1;
-            if (m == 0) ok = mbarWait(full + 8 * (seq % R), (seq / R) & 1, abortP, 5);
-            if (ok && m == 0 && j == tiles && clean) ok = mbarWait(vClean, 0, abortP, 6);
-            if (ok) ok = mbarWait(pReady + 8 * m, (j - 1) & 1, abortP, 7);
-            if (!ok) break;
-            values(m, j - 1);
-            if (m == tilesM - 1) tcCommit(empty + 8 * (seq % R));
-            if (j == tiles) tcCommit(oFull + 8 * m);
+            ok = mbarWait(full + 8 * slot, phase, abortP, 5);
+            if (ok && j == tiles && clean) ok = mbarWait(vClean, 0, abortP, 6);
+            advance();
           }
-          if (j < tiles) {
-            scores(m, j);
-            if (m == tilesM - 1) tcCommit(empty + 8 * (2 * j % R));
+          const int kSlot = slot;
+          if (ok && j < tiles) {
+            ok = mbarWait(full + 8 * slot, phase, abortP, 4);
+            advance();
+          }
+          const uint32_t vLow = (ringLow + vSlot * (TILE >> 4)) | apart, kLow = ringLow + kSlot * (TILE >> 4);
+          for (int m = 0; ok && m < tilesM; ++m) {
+            const uint32_t sCol = tmemBase + m * AW_KEYS, oCol = tmemBase + 2 * AW_KEYS + m * D;
+            if (j > 0) { // O_m += P_m V: steps of 16 keys as each half of the probabilities arrives; P from tensor memory, V MN-major
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                ok = ok && mbarWait(pReady + 16 * m + 8 * h, (j - 1) & 1, abortP, 7);
+                if (ok) {
+                  tcFenceAfter();
+#pragma unroll
+                  for (int ks = 4 * h; ks < 4 * h + 4; ++ks) tcMmaTmemA(oCol, sCol + ks * 8, desc(vLow + ks * (2048 >> 4)), idPV, (j > 1) | (ks > 0));
+                }
+              }
+              if (!ok) break;
+              if (m == tilesM - 1) tcCommit(empty + 8 * vSlot);
+              if (j == tiles) tcCommit(oFull + 8 * m);
+            }
+            if (j < tiles) { // S_m = Q_m K^T: steps of 16 along d, both operands K-major
+              const uint32_t aLow = qLow + m * (TILE >> 4);
+              tcFenceAfter();
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks) {
+                const uint32_t off = ((ks >> 2) * COLS + (ks & 3) * 32) >> 4;
+                tcMma(sCol, desc(aLow + off), desc(kLow + off), idS, ks > 0);
+              }
+              tcCommit(sFull + 8 * m);
+              if (m == tilesM - 1) tcCommit(empty + 8 * kSlot);
+            }
           }
         }
       }
     }
-  } else if ((warp - 2) >> 2 < tilesM) {
-    const int m = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane; // TMEM lanes are reachable by warp id mod 4
-    const int qi = q0 + m * perTile + row / p.Gp, pos = p.offset + qi;
-    const int tMin = p.offset + q0 + m * perTile, tMax = tMin + perTile - 1; // positions of this row tile
-    const uint32_t laneAddr = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t sAddr = laneAddr + m * AW_KEYS, oAddr = laneAddr + 2 * AW_KEYS + m * D;
-    const float sl2 = p.scaleLog2;
-    // `ref` is the maximum the exponentials are taken against; it follows the true one only when that has grown by more
-    // than a factor 2^8 (probabilities stay below 2^8), so that most tiles leave O alone.
-    float ref = -INFINITY, l = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
-      if (!__all_sync(0xffffffffu, mbarWait(sFull + 8 * m, j & 1, abortP, 8))) { ok = false; break; }
-      tcFenceAfter();
-      uint32_t sc[4][32];
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if ((warp - 4) >> 2 < tilesM) {
+      const int m = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane; // TMEM lanes are reachable by warp id mod 4
+      const int qi = q0 + m * perTile + row / p.Gp, pos = p.offset + qi;
+      const int tMin = p.offset + q0 + m * perTile, tMax = tMin + perTile - 1; // positions of this row tile
+      const uint32_t laneAddr = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t sAddr = laneAddr + m * AW_KEYS, oAddr = laneAddr + 2 * AW_KEYS + m * D;
+      const float sl2 = p.scaleLog2;
+      // `ref` is the maximum the exponentials are taken against; it follows the true one only when that has grown by more
+      // than a factor 2^8 (probabilities stay below 2^8), so that most tiles leave O alone.
+      float ref = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j) {
+        if (!__all_sync(0xffffffffu, mbarWait(sFull + 8 * m, j & 1, abortP, 8))) { ok = false; break; }
+        tcFenceAfter();
+        uint32_t sc[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tcLoad32(sAddr + c * 32, sc[c]);
-      // Visible keys of this row in each run, relative to its first key: lo .. hi.
-      int lo[2], hi[2];
-      bool mask = false;
+        for (int c = 0; c < 4; ++c) tcLoad32(sAddr + c * 32, sc[c]);
+        // Visible keys of this row in each run, relative to its first key: lo .. hi.
+        int lo[2], hi[2];
+        bool mask = false;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int run = 2 * j + h;
-        if (run < sinkRuns) {
-          lo[h] = 0;
-          hi[h] = min(pos, sinkN - 1) - run * AW_RUN;
-          mask |= min(tMin, sinkN - 1) < run * AW_RUN + AW_RUN - 1;
-        } else if (run < runs) {
-          const int key0 = start + (run - sinkRuns) * AW_RUN;
-          lo[h] = pos - p.window + 1 - key0;
-          hi[h] = min(pos, n - 1) - key0;
-          mask |= tMax - p.window + 1 > key0 || min(tMin, n - 1) < key0 + AW_RUN - 1;
-        } else {
-          lo[h] = 1;
-          hi[h] = 0;
-          mask = true;
+        for (int h = 0; h < 2; ++h) {
+          const int run = 2 * j + h;
+          if (run < sinkRuns) {
+            lo[h] = 0;
+            hi[h] = min(pos, sinkN - 1) - run * AW_RUN;
+            mask |= min(tMin, sinkN - 1) < run * AW_RUN + AW_RUN - 1;
+          } else if (run < runs) {
+            const int key0 = start + (run - sinkRuns) * AW_RUN;
+            lo[h] = pos - p.window + 1 - key0;
+            hi[h] = min(pos, n - 1) - key0;
+            mask |= tMax - p.window + 1 > key0 || min(tMin, n - 1) < key0 + AW_RUN - 1;
+          } else {
+            lo[h] = 1;
+            hi[h] = 0;
+            mask = true;
+          }
         }
-      }
-      tcWaitLd();
-      if (mask) {
+        tcWaitLd();
+        if (mask) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int at = (c & 1) * 32 + i;
+              if (at < lo[c >> 1] || at > hi[c >> 1]) sc[c][i] = 0xff800000u; // -inf
+            }
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int at = (c & 1) * 32 + i;
-            if (at < lo[c >> 1] || at > hi[c >> 1]) sc[c][i] = 0xff800000u; // -inf
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], __uint_as_float(sc[c][i + k]), __uint_as_float(sc[c][i + 4 + k]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        float corr = 1.0f;
+        if (ref == -INFINITY) {
+          ref = mx; // nothing was seen so far: O and l are zero
+        } else if ((mx - ref) * sl2 > 8.0f) {
+          corr = fastExp2((ref - mx) * sl2);
+          ref = mx;
+        }
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+          // The scores of this tile were issued behind P V of the one before: O is complete.
+          l *= corr;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            tcLoad32(oAddr + c * 32, r);
+            tcWaitLd();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+            tcStore32(oAddr + c * 32, r);
           }
+        }
+        const float negM = ref == -INFINITY ? 0.0f : -ref * sl2;
+        const uint64_t sl2x2 = pack2(sl2, sl2), negMx2 = pack2(negM, negM);
+        uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int at = c * 64 + 2 * i;
+            float x, y;
+            unpack2(fma2(pack2u(sc[at >> 5][at & 31], sc[at >> 5][(at & 31) + 1]), sl2x2, negMx2), x, y);
+            x = fastExp2(x);
+            y = fastExp2(y);
+            sum[i & 1] = add2(sum[i & 1], pack2(x, y));
+            w[i] = packPair<T>(x, y);
+          }
+          tcStore32(sAddr + c * 32, w);
+          tcWaitSt();
+          tcFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArrive(pReady + 16 * m + 8 * c);
+        }
+        float s0, s1, s2, s3;
+        unpack2(sum[0], s0, s1);
+        unpack2(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
       }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], __uint_as_float(sc[c][i + k]), __uint_as_float(sc[c][i + 4 + k]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-      float corr = 1.0f;
-      if (ref == -INFINITY) {
-        ref = mx; // nothing was seen so far: O and l are zero
-      } else if ((mx - ref) * sl2 > 8.0f) {
-        corr = fastExp2((ref - mx) * sl2);
-        ref = mx;
-      }
-      if (__any_sync(0xffffffffu, corr != 1.0f)) {
-        // The scores of this tile were issued behind P V of the one before: O is complete.
-        l *= corr;
+      if (ok && tiles > 0 && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * m, 0, abortP, 9))) ok = false;
+      if (ok) {
+        tcFenceAfter();
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        T *orow = out + b * p.ob + (head0 + row % p.Gp) * p.oh + qi * p.os;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
-          tcLoad32(oAddr + c * 32, r);
-          tcWaitLd();
+          if (tiles > 0) {
+            tcLoad32(oAddr + c * 32, r);
+            tcWaitLd();
+          }
+          if (qi < p.Sq) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
-          tcStore32(oAddr + c * 32, r);
-        }
-      }
-      const float negM = ref == -INFINITY ? 0.0f : -ref * sl2;
-      const uint64_t sl2x2 = pack2(sl2, sl2), negMx2 = pack2(negM, negM);
-      uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int at = c * 64 + 2 * i;
-          float x, y;
-          unpack2(fma2(pack2u(sc[at >> 5][at & 31], sc[at >> 5][(at & 31) + 1]), sl2x2, negMx2), x, y);
-          x = fastExp2(x);
-          y = fastExp2(y);
-          sum[i & 1] = add2(sum[i & 1], pack2(x, y));
-          w[i] = packPair<T>(x, y);
-        }
-        tcStore32(sAddr + c * 32, w);
-      }
-      tcWaitSt();
-      tcFenceBefore();
-      float s0, s1, s2, s3;
-      unpack2(sum[0], s0, s1);
-      unpack2(sum[1], s2, s3);
-      l += (s0 + s1) + (s2 + s3);
-      __syncwarp();
-      if (lane == 0) mbarArrive(pReady + 8 * m);
-    }
-    if (ok && tiles > 0 && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * m, 0, abortP, 9))) ok = false;
-    if (ok) {
-      tcFenceAfter();
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      T *orow = out + b * p.ob + (head0 + row % p.Gp) * p.oh + qi * p.os;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        if (tiles > 0) {
-          tcLoad32(oAddr + c * 32, r);
-          tcWaitLd();
-        }
-        if (qi < p.Sq) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 v = make_uint4(0, 0, 0, 0); // a row that sees no key (O may never have been written)
-            if (l > 0.0f) {
-              v.x = packPair<T>(__uint_as_float(r[g * 8]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
-              v.y = packPair<T>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
-              v.z = packPair<T>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
-              v.w = packPair<T>(__uint_as_float(r[g * 8 + 6]) * inv, __uint_as_float(r[g * 8 + 7]) * inv);
+            for (int g = 0; g < 4; ++g) {
+              uint4 v = make_uint4(0, 0, 0, 0); // a row that sees no key (O may never have been written)
+              if (l > 0.0f) {
+                v.x = packPair<T>(__uint_as_float(r[g * 8]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
+                v.y = packPair<T>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
+                v.z = packPair<T>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
+                v.w = packPair<T>(__uint_as_float(r[g * 8 + 6]) * inv, __uint_as_float(r[g * 8 + 7]) * inv);
+              }
+              *reinterpret_cast<uint4 *>(orow + c * 32 + g * 8) = v;
             }
-            *reinterpret_cast<uint4 *>(orow + c * 32 + g * 8) = v;
           }
         }
       }
