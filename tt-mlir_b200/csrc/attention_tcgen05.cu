@@ -901,6 +901,7 @@ int sdpaTcgen05Try(const void *q, const void *k, const void *v, void *out, int d
 } // namespace ttb
 
 #include "attention_window_tcgen05.cuh"
+#include "attention_cached_tcgen05.cuh"
 
 namespace ttb {
 // Reads and / or writes this file's copies of the status word and the wait limit (current device).

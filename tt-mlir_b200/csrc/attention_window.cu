@@ -16,6 +16,7 @@
 // tile into WM groups of rows and 4 / WM groups of keys, each with its own running maximum and sum, merged at the
 // end through shared memory.  One row tile per kv head is bound by HBM (16 rows: 16 multiply-adds per byte read).
 // With few users the slots are split over `splits` CTAs and a second kernel joins the parts.
+#include "attention_cached.cuh"
 #include "common.cuh"
 
 #include <algorithm>
@@ -529,6 +530,35 @@ static int windowSplits(int64_t batch, int64_t kvHeads, int64_t rows, int64_t ma
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, 128})));
 }
 
+// How a tree's rows are computed, from the sizes that its workspace is asked for with.
+struct TreePlan {
+  bool tall;  // tensor-core kernel with 128-row tiles
+  int splits; // runs of slots per row tile
+  int parts;  // partial results per row (1: none, the result itself)
+};
+static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kvHeads, int64_t dim, int64_t positions) {
+  const int64_t rows = nodes * (heads / kvHeads), slots = positions + nodes;
+  TreePlan t;
+  t.tall = rows > 32 && (dim == 64 || dim == 128);
+  if (!t.tall) {
+    t.parts = t.splits = windowSplits(batch, kvHeads, rows, slots);
+    return t;
+  }
+  // One CTA per SM: waves x (tiles per CTA + 6 for what a CTA costs besides), at the longest possible length.
+  const int64_t base = batch * kvHeads * ((rows + 127) / 128), tiles = (slots + 127) / 128;
+  int64_t best = 0;
+  t.splits = 1;
+  for (int64_t s = 1; s <= std::min<int64_t>(64, std::max<int64_t>(1, tiles / 2)); ++s) {
+    const int64_t cost = (base * s + smCount() - 1) / smCount() * ((tiles + s - 1) / s + 6);
+    if (s == 1 || cost < best) {
+      best = cost;
+      t.splits = static_cast<int>(s);
+    }
+  }
+  t.parts = 2 * t.splits;
+  return t;
+}
+
 static size_t windowPartBytes(int64_t batch, int64_t nq, int64_t heads, int64_t dim, int64_t splits) {
   if (splits <= 1) return 0;
   return static_cast<size_t>(batch) * nq * heads * splits * (dim + 2) * sizeof(float);
@@ -536,6 +566,15 @@ static size_t windowPartBytes(int64_t batch, int64_t nq, int64_t heads, int64_t 
 
 static int64_t maxVisible(int64_t keys, int64_t window, int64_t sinks) {
   return window > 0 && window < keys - sinks ? window + sinks : keys;
+}
+
+// Joins the p.splits parts of every row.
+template <typename T, int D> static int launchWindowJoin(void *out, const WindowParams &p, cudaStream_t st) {
+  const int64_t all = static_cast<int64_t>(p.batch) * p.nq * p.heads;
+  TTB_CUDA(launchPdl(windowJoinKernel<T, D>, dim3(static_cast<unsigned>((all + 3) / 4)), dim3(128), 0, st, static_cast<T *>(out), p, all));
+  countLaunch();
+  TTB_LAUNCH_CHECK();
+  return TTB_OK;
 }
 
 template <typename T, int D, int WM>
@@ -555,13 +594,8 @@ static int launchWindowMma(const void *q, const void *k, const void *v, const vo
   TTB_CUDA(launchPdl(windowMmaKernel<T, D, WM>, grid, dim3(WN_THREADS), smem, st, static_cast<const T *>(q), static_cast<const T *>(k),
                      static_cast<const T *>(v), static_cast<const T *>(kd), static_cast<const T *>(vd), static_cast<T *>(out), p));
   countLaunch();
-  if (p.splits > 1) {
-    const int64_t all = static_cast<int64_t>(p.batch) * p.nq * p.heads;
-    TTB_CUDA(launchPdl(windowJoinKernel<T, D>, dim3(static_cast<unsigned>((all + 3) / 4)), dim3(128), 0, st, static_cast<T *>(out), p, all));
-    countLaunch();
-  }
   TTB_LAUNCH_CHECK();
-  return TTB_OK;
+  return p.splits > 1 ? launchWindowJoin<T, D>(out, p, st) : TTB_OK;
 }
 
 template <typename T, int D>
@@ -746,8 +780,7 @@ int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const vo
 
 size_t ttb_sdpa_tree_workspace_bytes(int batch, int nodes, int heads, int kv_heads, int head_dim, int64_t positions) {
   if (batch <= 0 || nodes <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || positions <= 0 || heads % kv_heads) return 0;
-  const int64_t rows = static_cast<int64_t>(nodes) * (heads / kv_heads);
-  return windowPartBytes(batch, nodes, heads, head_dim, windowSplits(batch, kv_heads, rows, positions + nodes));
+  return windowPartBytes(batch, nodes, heads, head_dim, treePlan(batch, nodes, heads, kv_heads, head_dim, positions).parts);
 }
 
 int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const void *k_cache, const void *v_cache, const void *page_table,
@@ -775,7 +808,8 @@ int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const
   p.qs = p.os = static_cast<int64_t>(heads) * head_dim;
   p.qh = p.oh = head_dim;
   // The workspace must not depend on the window (its size is asked for without one), so neither do the splits.
-  p.splits = windowSplits(batch, kv_heads, static_cast<int64_t>(nodes) * p.G, positions + nodes);
+  const TreePlan plan = treePlan(batch, nodes, heads, kv_heads, head_dim, positions);
+  p.splits = plan.parts;
   const size_t need = windowPartBytes(batch, nodes, heads, head_dim, p.splits);
   TTB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (see ttb_sdpa_tree_workspace_bytes)");
   const int flagged = indexBadFlag(&p.bad);
@@ -788,6 +822,20 @@ int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const
   const double slots = double(maxVisible(positions, window, sinks)) + nodes; // an upper bound
   ProfScope prof("sdpa_tree", 4.0 * batch * nodes * heads * slots * head_dim,
                  4.0 * batch * kv_heads * slots * head_dim + 4.0 * batch * nodes * heads * head_dim, st);
+  if (plan.tall && p.scaleLog2 > 0.0f) {
+    AcParams a = {};
+    a.table = p.table; a.lens = p.lens; a.parents = p.parents; a.draftLen = p.draftLen; a.bad = p.bad;
+    a.pages = p.pages; a.blockSize = p.blockSize; a.blocks = p.blocks; a.parentsUsers = p.parentsUsers;
+    a.nq = p.nq; a.heads = p.heads; a.kvHeads = p.kvHeads; a.G = p.G; a.keys = p.keys; a.window = p.window; a.sinks = p.sinks;
+    a.splits = plan.splits;
+    a.fmt = dtype == kBF16 ? 1 : 0;
+    a.scaleLog2 = p.scaleLog2;
+    a.pm = p.pm; a.pl = p.pl; a.po = p.po;
+    const int rc2 = sdpaCachedTcgen05(q, k_cache, v_cache, k_draft, v_draft, dtype, head_dim, batch, a, st);
+    if (rc2) return rc2;
+    if (dtype == kBF16) return head_dim == 64 ? launchWindowJoin<__nv_bfloat16, 64>(out, p, st) : launchWindowJoin<__nv_bfloat16, 128>(out, p, st);
+    return head_dim == 64 ? launchWindowJoin<__half, 64>(out, p, st) : launchWindowJoin<__half, 128>(out, p, st);
+  }
   if (dtype == kBF16) return windowMma<__nv_bfloat16>(q, k_cache, v_cache, k_draft, v_draft, out, head_dim, p, st);
   return windowMma<__half>(q, k_cache, v_cache, k_draft, v_draft, out, head_dim, p, st);
 }

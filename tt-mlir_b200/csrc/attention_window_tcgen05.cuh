@@ -47,6 +47,68 @@ struct AwParams {
   float scaleLog2;
 };
 
+// One row's share of a 128-key tile, by one thread: `sc` are its scores (-inf where masked).  `ref` is the maximum the
+// exponentials are taken against; it follows the true one only when that has grown by more than a factor 2^8
+// (probabilities stay below 2^8), so that most tiles leave O alone.  The probabilities, rounded to T, go over the first
+// half of the columns of the scores at sAddr, ready(half) after each half of them; `l` gathers their sum before rounding.
+template <typename T, int D, typename Ready>
+__device__ __forceinline__ void awSoftmax(uint32_t (&sc)[4][32], uint32_t sAddr, uint32_t oAddr, float sl2, float &ref, float &l, Ready &&ready) {
+  float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], __uint_as_float(sc[c][i + k]), __uint_as_float(sc[c][i + 4 + k]));
+  const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+  float corr = 1.0f;
+  if (ref == -INFINITY) {
+    ref = mx; // nothing was seen so far: O and l are zero
+  } else if ((mx - ref) * sl2 > 8.0f) {
+    corr = fastExp2((ref - mx) * sl2);
+    ref = mx;
+  }
+  if (__any_sync(0xffffffffu, corr != 1.0f)) {
+    // The scores of this tile were issued behind P V of the one before: O is complete.
+    l *= corr;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t r[32];
+      tcLoad32(oAddr + c * 32, r);
+      tcWaitLd();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+      tcStore32(oAddr + c * 32, r);
+    }
+  }
+  const float negM = ref == -INFINITY ? 0.0f : -ref * sl2;
+  const uint64_t sl2x2 = pack2(sl2, sl2), negMx2 = pack2(negM, negM);
+  uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int at = c * 64 + 2 * i;
+      float x, y;
+      unpack2(fma2(pack2u(sc[at >> 5][at & 31], sc[at >> 5][(at & 31) + 1]), sl2x2, negMx2), x, y);
+      x = fastExp2(x);
+      y = fastExp2(y);
+      sum[i & 1] = add2(sum[i & 1], pack2(x, y));
+      w[i] = packPair<T>(x, y);
+    }
+    tcStore32(sAddr + c * 32, w);
+    tcWaitSt();
+    tcFenceBefore();
+    __syncwarp();
+    ready(c);
+  }
+  float s0, s1, s2, s3;
+  unpack2(sum[0], s0, s1);
+  unpack2(sum[1], s2, s3);
+  l += (s0 + s1) + (s2 + s3);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(AW_THREADS, 1)
     sdpaWindowTcgen05Kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
@@ -226,8 +288,6 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
       const uint32_t laneAddr = tmemBase + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t sAddr = laneAddr + m * AW_KEYS, oAddr = laneAddr + 2 * AW_KEYS + m * D;
       const float sl2 = p.scaleLog2;
-      // `ref` is the maximum the exponentials are taken against; it follows the true one only when that has grown by more
-      // than a factor 2^8 (probabilities stay below 2^8), so that most tiles leave O alone.
       float ref = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
@@ -267,60 +327,9 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
               if (at < lo[c >> 1] || at > hi[c >> 1]) sc[c][i] = 0xff800000u; // -inf
             }
         }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], __uint_as_float(sc[c][i + k]), __uint_as_float(sc[c][i + 4 + k]));
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        float corr = 1.0f;
-        if (ref == -INFINITY) {
-          ref = mx; // nothing was seen so far: O and l are zero
-        } else if ((mx - ref) * sl2 > 8.0f) {
-          corr = fastExp2((ref - mx) * sl2);
-          ref = mx;
-        }
-        if (__any_sync(0xffffffffu, corr != 1.0f)) {
-          // The scores of this tile were issued behind P V of the one before: O is complete.
-          l *= corr;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            tcLoad32(oAddr + c * 32, r);
-            tcWaitLd();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
-            tcStore32(oAddr + c * 32, r);
-          }
-        }
-        const float negM = ref == -INFINITY ? 0.0f : -ref * sl2;
-        const uint64_t sl2x2 = pack2(sl2, sl2), negMx2 = pack2(negM, negM);
-        uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int at = c * 64 + 2 * i;
-            float x, y;
-            unpack2(fma2(pack2u(sc[at >> 5][at & 31], sc[at >> 5][(at & 31) + 1]), sl2x2, negMx2), x, y);
-            x = fastExp2(x);
-            y = fastExp2(y);
-            sum[i & 1] = add2(sum[i & 1], pack2(x, y));
-            w[i] = packPair<T>(x, y);
-          }
-          tcStore32(sAddr + c * 32, w);
-          tcWaitSt();
-          tcFenceBefore();
-          __syncwarp();
-          if (lane == 0) mbarArrive(pReady + 16 * m + 8 * c);
-        }
-        float s0, s1, s2, s3;
-        unpack2(sum[0], s0, s1);
-        unpack2(sum[1], s2, s3);
-        l += (s0 + s1) + (s2 + s3);
+        awSoftmax<T, D>(sc, sAddr, oAddr, sl2, ref, l, [&](int half) {
+          if (lane == 0) mbarArrive(pReady + 16 * m + 8 * half);
+        });
       }
       if (ok && tiles > 0 && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * m, 0, abortP, 9))) ok = false;
       if (ok) {
