@@ -10,6 +10,7 @@ struct AcParams { // pointers and sizes as in ttb_sdpa_tree; window and sinks al
   int *bad;
   int pages, blockSize, blocks, parentsUsers;
   int nq, heads, kvHeads, G, keys, window, sinks, splits, fmt;
+  int boxes; // set by the launcher: the cache has tensor maps
   float scaleLog2;
   float *pm, *pl, *po;
 };

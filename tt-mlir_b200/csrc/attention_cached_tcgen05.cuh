@@ -3,13 +3,14 @@
 // Part of attention_tcgen05.cu, whose status word it shares.
 //
 // One CTA owns 128 rows (node, head of the group) of a (user, kv head) and a run of slots, in tiles of 128:
-//   warps 0..3    fetch: each warp 32 slots of a tile, whose rows it looks up (pages, drafts) and copies with cp.async into
-//                 the swizzled operand layout; a slot that no row sees is filled with zeros
+//   warps 0..3    fetch: each warp 32 slots of a tile.  When those are 32 neighbouring rows of one page, four TMA boxes
+//                 bring them; otherwise (pages that end inside, a window's odd start, drafts, the ragged end) the warp looks
+//                 every row up and copies it with cp.async into the swizzled operand layout, zeros for a slot that no row
+//                 sees
 //   warps 4..7, 8..11  softmax of the even and of the odd tiles, one row per thread
 //   warp 12       issues tcgen05.mma
 // Even and odd tiles are two chains of their own (scores, probabilities, output and maximum), so that one chain's softmax
-// runs beside the other's products; their two outputs are two partial results for the joining kernel.  cp.async rather
-// than TMA: pages may have any size, a window starts anywhere, and rows must read as zero at any slot.
+// runs beside the other's products; their two outputs are two partial results for the joining kernel.
 // Bound: HBM as long as a tile of keys and values (64 KB at head_dim 128) takes longer to arrive than a chain's round trip.
 #pragma once
 
@@ -28,8 +29,8 @@ template <int D> struct AcShape {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(AC_THREADS, 1)
-    sdpaCachedTcgen05Kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ kd,
-                            const T *__restrict__ vd, AcParams p) {
+    sdpaCachedTcgen05Kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const T *__restrict__ q,
+                            const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ kd, const T *__restrict__ vd, AcParams p) {
   using Sh = AcShape<D>;
   constexpr int R = Sh::STAGES, TILE = Sh::TILE, COLS = Sh::COLS, CPR = D / 8;
   extern __shared__ unsigned char smemRaw[];
@@ -157,21 +158,47 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         at = ((static_cast<int64_t>(b) * p.nq + (slot - cached)) * p.kvHeads + kvh) * D;
         return 2;
       };
-      int64_t at = 0;
-      int kind = find(s0 + warp * 32 + lane, at);
+      // The warp's 32 slots of tile j as one box: its block and first row in it, or -1.
+      auto box = [&](int j, int &in) -> int {
+        const int first = s0 + j * 128 + warp * 32;
+        if (!p.boxes || first + 32 > min(s1, cached) || (first < sinkN && first + 32 > sinkN)) return -1;
+        const int pos = first < sinkN ? first : start + (first - sinkN);
+        in = p.table ? pos % p.blockSize : pos;
+        if (in + 32 > p.blockSize) return -1;
+        if (!p.table) return b;
+        const int blk = p.table[static_cast<int64_t>(b) * p.pages + pos / p.blockSize];
+        return blk < 0 ? 0 : (blk >= p.blocks ? p.blocks - 1 : blk);
+      };
+      int in = 0, blk = box(0, in);
+      uint32_t boxed = 0; // bit i: the tile i steps back came by TMA, which has signalled it already
       bool ok = true;
       int stage = 0, phase = 0;
       for (int j = 0; j < tiles + Sh::LAG; ++j) {
+        boxed <<= 1;
         if (j < tiles) {
           if (!__all_sync(0xffffffffu, mbarWait(empty + 8 * stage, phase ^ 1, abortP, 1))) { ok = false; break; }
           const uint32_t kTile = sRing + 2 * stage * TILE;
-          rows(kTile, kind == 0 ? nullptr : (kind == 1 ? k : kd) + at, k);
-          rows(kTile + TILE, kind == 0 ? nullptr : (kind == 1 ? v : vd) + at, v);
+          if (blk >= 0) {
+            if (lane == 0) {
+              mbarArriveExpectTx(full + 8 * stage, 2 * 32 * D * 2);
+              for (int c = 0; c < D / 64; ++c) {
+                tmaLoad4d(kTile + c * COLS + warp * 4096, &mapK, full + 8 * stage, c * 64, in, kvh, blk);
+                tmaLoad4d(kTile + TILE + c * COLS + warp * 4096, &mapV, full + 8 * stage, c * 64, in, kvh, blk);
+              }
+            }
+            __syncwarp();
+            boxed |= 1u;
+          } else {
+            int64_t at = 0;
+            const int kind = find(s0 + j * 128 + warp * 32 + lane, at);
+            rows(kTile, kind == 0 ? nullptr : (kind == 1 ? k : kd) + at, k);
+            rows(kTile + TILE, kind == 0 ? nullptr : (kind == 1 ? v : vd) + at, v);
+          }
           if (++stage == R) {
             stage = 0;
             phase ^= 1;
           }
-          kind = find(s0 + (j + 1) * 128 + warp * 32 + lane, at); // the next tile's rows, while this one's are on their way
+          blk = j + 1 < tiles ? box(j + 1, in) : -1; // the next tile's page, while this one's rows are on their way
         }
         commit();
         if (j == 0) { // the queries came with the first group
@@ -180,7 +207,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         }
         if (j >= Sh::LAG) {
           asm volatile("cp.async.wait_group %0;" ::"n"(Sh::LAG) : "memory");
-          handOver(full + 8 * ((j - Sh::LAG) % R));
+          if (!(boxed >> Sh::LAG & 1u)) handOver(full + 8 * ((j - Sh::LAG) % R));
         }
       }
       (void)ok;
@@ -306,7 +333,12 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
 }
 
 template <typename T, int D>
-static int launchCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, int batch, const AcParams &p, cudaStream_t st) {
+static int launchCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, int batch, AcParams p, cudaStream_t st) {
+  // The cache as [blocks, kv heads, block size, D] in boxes of 32 rows; without one every row is copied on its own.
+  CUtensorMap mapK = {}, mapV = {};
+  const int64_t extents[4] = {D, p.blockSize, p.kvHeads, p.blocks}, row = D, head = row * p.blockSize, strides[3] = {row, head, head * p.kvHeads};
+  const int boxRows[3] = {32, 1, 1}, dtype = p.fmt ? kBF16 : kF16;
+  p.boxes = p.blockSize >= 32 && makeWindowMap(&mapK, k, dtype, extents, strides, boxRows) && makeWindowMap(&mapV, v, dtype, extents, strides, boxRows);
   static bool attrSet[64] = {}; // function attributes belong to a device
   int dev = 0;
   TTB_CUDA(cudaGetDevice(&dev));
@@ -317,8 +349,8 @@ static int launchCachedTcgen05(const void *q, const void *k, const void *v, cons
   const int64_t mts = (static_cast<int64_t>(p.nq) * p.G + 127) / 128;
   TTB_CHECK(mts * p.splits <= 0x7fffffff, "too many query rows");
   dim3 grid(static_cast<unsigned>(mts * p.splits), static_cast<unsigned>(p.kvHeads), static_cast<unsigned>(batch));
-  TTB_CUDA(launchPdl(sdpaCachedTcgen05Kernel<T, D>, grid, dim3(AC_THREADS), AcShape<D>::SMEM, st, static_cast<const T *>(q),
-                     static_cast<const T *>(k), static_cast<const T *>(v), static_cast<const T *>(kd), static_cast<const T *>(vd), p));
+  TTB_CUDA(launchPdl(sdpaCachedTcgen05Kernel<T, D>, grid, dim3(AC_THREADS), AcShape<D>::SMEM, st, mapK, mapV,
+                     static_cast<const T *>(q), static_cast<const T *>(k), static_cast<const T *>(v), static_cast<const T *>(kd), static_cast<const T *>(vd), p));
   countLaunch();
   TTB_LAUNCH_CHECK();
   return TTB_OK;
