@@ -15,7 +15,7 @@ struct AcParams { // pointers and sizes as in ttb_sdpa_tree; window and sinks al
   float *pm, *pl, *po;
 };
 
-int sdpaCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, int dtype, int dim, int batch, const AcParams &p,
+int sdpaCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, void *out, int dtype, int dim, int batch, const AcParams &p,
                       cudaStream_t st);
 
 } // namespace ttb

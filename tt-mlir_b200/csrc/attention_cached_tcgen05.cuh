@@ -3,14 +3,14 @@
 // Part of attention_tcgen05.cu, whose status word it shares.
 //
 // One CTA owns 128 rows (node, head of the group) of a (user, kv head) and a run of slots, in tiles of 128:
-//   warps 0..3    fetch: each warp 32 slots of a tile.  When those are 32 neighbouring rows of one page, four TMA boxes
-//                 bring them; otherwise (pages that end inside, a window's odd start, drafts, the ragged end) the warp looks
-//                 every row up and copies it with cp.async into the swizzled operand layout, zeros for a slot that no row
-//                 sees
+//   warps 0..3    fetch, two of them keys and two values (a key tile is free as soon as its scores are there, long before
+//                 its values), each 64 slots of a tile.  32 neighbouring rows of one page come as TMA boxes; otherwise
+//                 (pages that end inside, a window's odd start, drafts, the ragged end) the warp looks every row up and
+//                 copies it with cp.async into the swizzled operand layout, zeros for a slot that no row sees
 //   warps 4..7, 8..11  softmax of the even and of the odd tiles, one row per thread
 //   warp 12       issues tcgen05.mma
 // Even and odd tiles are two chains of their own (scores, probabilities, output and maximum), so that one chain's softmax
-// runs beside the other's products; their two outputs are two partial results for the joining kernel.
+// runs beside the other's products; at the end the odd chain hands its output to the even one through the ring's memory.
 // Bound: HBM as long as a tile of keys and values (64 KB at head_dim 128) takes longer to arrive than a chain's round trip.
 #pragma once
 
@@ -24,13 +24,15 @@ template <int D> struct AcShape {
   static constexpr int COLS = 128 * 128;            // bytes of its 64-column part
   static constexpr int STAGES = D == 128 ? 3 : 6;   // K and V of one tile each
   static constexpr int LAG = STAGES - 2;            // tiles on their way behind the one handed over; one stage is being used up
-  static constexpr int SMEM = TILE + 2 * STAGES * TILE + 1024 /* alignment slack */ + 256 /* barriers */;
+  static constexpr int SMEM = TILE + 2 * STAGES * TILE + 1024 /* alignment slack */ + 512 /* barriers: 8 (4 STAGES + 10) */;
+  static_assert(2 * STAGES * TILE >= (D + 2) * 128 * 4, "the ring takes one chain's output, maxima and sums");
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(AC_THREADS, 1)
     sdpaCachedTcgen05Kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const T *__restrict__ q,
-                            const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ kd, const T *__restrict__ vd, AcParams p) {
+                            const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ kd, const T *__restrict__ vd, T *__restrict__ out,
+                            AcParams p) {
   using Sh = AcShape<D>;
   constexpr int R = Sh::STAGES, TILE = Sh::TILE, COLS = Sh::COLS, CPR = D / 8;
   extern __shared__ unsigned char smemRaw[];
@@ -41,16 +43,18 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
 
   const uint32_t base = (smemU32(smemRaw) + 1023u) & ~1023u;
   const uint32_t sQ = base, sRing = base + TILE, bars = sRing + 2 * R * TILE;
-  const uint32_t qFull = bars, full = bars + 8, empty = full + 8 * R, sFull = empty + 8 * R, pReady = sFull + 16 /* [chain][half] */,
-                 oFull = pReady + 32;
+  // full / empty: K tiles' barriers, then V tiles'
+  const uint32_t qFull = bars, full = bars + 8, empty = full + 16 * R, sFull = empty + 16 * R, pReady = sFull + 16 /* [chain][half] */,
+                 oFull = pReady + 32, handed = oFull + 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     abortFlag = 0;
     mbarInit(qFull, 4);
-    for (int i = 0; i < R; ++i) {
-      mbarInit(full + 8 * i, 4);
+    for (int i = 0; i < 2 * R; ++i) {
+      mbarInit(full + 8 * i, 2);
       mbarInit(empty + 8 * i, 1);
     }
+    mbarInit(handed, 4);
     for (int i = 0; i < 2; ++i) {
       mbarInit(sFull + 8 * i, 1);
       mbarInit(pReady + 16 * i, 4);
@@ -121,13 +125,13 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
     };
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    // 32 rows of a tile, one pointer per lane (null: zeros): two (D = 64: four) rows per instruction.
-    auto rows = [&](uint32_t tile, const T *mine, const T *any) {
+    // 32 rows of a tile from row `to` on, one pointer per lane (null: zeros): two (D = 64: four) rows per instruction.
+    auto rows = [&](uint32_t tile, int to, const T *mine, const T *any) {
       constexpr int PER = 32 / CPR;
       const int c = lane % CPR;
 #pragma unroll 4
       for (int i = 0; i < 32 / PER; ++i) {
-        const int from = i * PER + lane / CPR, row = warp * 32 + from;
+        const int from = i * PER + lane / CPR, row = to + from;
         const T *src = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), from));
         copy(tile + (c >> 3) * COLS + row * 128 + (((c & 7) ^ (row & 7)) << 4), src ? src + c * 8 : any, src != nullptr);
       }
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
     };
     if (tiles > 0) {
       const int row = r0 + warp * 32 + lane;
-      rows(sQ, row < p.nq * p.G ? q + ((static_cast<int64_t>(b) * p.nq + row / p.G) * p.heads + kvh * p.G + row % p.G) * D : nullptr, q);
+      rows(sQ, warp * 32, row < p.nq * p.G ? q + ((static_cast<int64_t>(b) * p.nq + row / p.G) * p.heads + kvh * p.G + row % p.G) * D : nullptr, q);
       commit();
       const int64_t kh = static_cast<int64_t>(p.blockSize) * D, kb = kh * p.kvHeads;
       auto find = [&](int slot, int64_t &at) -> int { // where the slot's row is: 0 nowhere, 1 in the cache, 2 among the drafts
@@ -158,9 +162,8 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         at = ((static_cast<int64_t>(b) * p.nq + (slot - cached)) * p.kvHeads + kvh) * D;
         return 2;
       };
-      // The warp's 32 slots of tile j as one box: its block and first row in it, or -1.
-      auto box = [&](int j, int &in) -> int {
-        const int first = s0 + j * 128 + warp * 32;
+      // 32 slots from `first` on as one box: its block and first row in it, or -1.
+      auto box = [&](int first, int &in) -> int {
         if (!p.boxes || first + 32 > min(s1, cached) || (first < sinkN && first + 32 > sinkN)) return -1;
         const int pos = first < sinkN ? first : start + (first - sinkN);
         in = p.table ? pos % p.blockSize : pos;
@@ -169,36 +172,42 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         const int blk = p.table[static_cast<int64_t>(b) * p.pages + pos / p.blockSize];
         return blk < 0 ? 0 : (blk >= p.blocks ? p.blocks - 1 : blk);
       };
-      int in = 0, blk = box(0, in);
-      uint32_t boxed = 0; // bit i: the tile i steps back came by TMA, which has signalled it already
-      bool ok = true;
+      const bool value = warp >= 2;
+      const int to = (warp & 1) * 64; // this warp's rows of a tile
+      const CUtensorMap *map = value ? &mapV : &mapK;
+      const T *cache = value ? v : k, *drafts = value ? vd : kd;
+      const uint32_t fullB = full + (value ? 8 * R : 0), emptyB = empty + (value ? 8 * R : 0);
+      int in[2] = {0, 0}, blk[2];
+      for (int h = 0; h < 2; ++h) blk[h] = box(s0 + to + 32 * h, in[h]);
+      uint32_t arrived = 0; // bit i: the tile i steps back had boxes only, and has been signalled
       int stage = 0, phase = 0;
       for (int j = 0; j < tiles + Sh::LAG; ++j) {
-        boxed <<= 1;
+        arrived <<= 1;
         if (j < tiles) {
-          if (!__all_sync(0xffffffffu, mbarWait(empty + 8 * stage, phase ^ 1, abortP, 1))) { ok = false; break; }
-          const uint32_t kTile = sRing + 2 * stage * TILE;
-          if (blk >= 0) {
-            if (lane == 0) {
-              mbarArriveExpectTx(full + 8 * stage, 2 * 32 * D * 2);
-              for (int c = 0; c < D / 64; ++c) {
-                tmaLoad4d(kTile + c * COLS + warp * 4096, &mapK, full + 8 * stage, c * 64, in, kvh, blk);
-                tmaLoad4d(kTile + TILE + c * COLS + warp * 4096, &mapV, full + 8 * stage, c * 64, in, kvh, blk);
+          if (!__all_sync(0xffffffffu, mbarWait(emptyB + 8 * stage, phase ^ 1, abortP, 1))) break;
+          const uint32_t tile = sRing + (2 * stage + (value ? 1 : 0)) * TILE, bar = fullB + 8 * stage;
+          for (int h = 0; h < 2; ++h) {
+            if (blk[h] >= 0) {
+              if (lane == 0) { // this warp's arrival is still due, so the phase cannot end before the bytes are expected
+                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(32 * D * 2) : "memory");
+                for (int c = 0; c < D / 64; ++c) tmaLoad4d(tile + c * COLS + (to + 32 * h) * 128, map, bar, c * 64, in[h], kvh, blk[h]);
               }
+              __syncwarp();
+            } else {
+              int64_t at = 0;
+              const int kind = find(s0 + j * 128 + to + 32 * h + lane, at);
+              rows(tile, to + 32 * h, kind == 0 ? nullptr : (kind == 1 ? cache : drafts) + at, cache);
             }
-            __syncwarp();
-            boxed |= 1u;
-          } else {
-            int64_t at = 0;
-            const int kind = find(s0 + j * 128 + warp * 32 + lane, at);
-            rows(kTile, kind == 0 ? nullptr : (kind == 1 ? k : kd) + at, k);
-            rows(kTile + TILE, kind == 0 ? nullptr : (kind == 1 ? v : vd) + at, v);
+          }
+          if (blk[0] >= 0 && blk[1] >= 0) {
+            if (lane == 0) mbarArrive(bar);
+            arrived |= 1u;
           }
           if (++stage == R) {
             stage = 0;
             phase ^= 1;
           }
-          blk = j + 1 < tiles ? box(j + 1, in) : -1; // the next tile's page, while this one's rows are on their way
+          for (int h = 0; h < 2; ++h) blk[h] = j + 1 < tiles ? box(s0 + (j + 1) * 128 + to + 32 * h, in[h]) : -1; // the next tile's pages
         }
         commit();
         if (j == 0) { // the queries came with the first group
@@ -207,10 +216,9 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         }
         if (j >= Sh::LAG) {
           asm volatile("cp.async.wait_group %0;" ::"n"(Sh::LAG) : "memory");
-          if (!(boxed >> Sh::LAG & 1u)) handOver(full + 8 * ((j - Sh::LAG) % R));
+          if (!(arrived >> Sh::LAG & 1u)) handOver(fullB + 8 * ((j - Sh::LAG) % R));
         }
       }
-      (void)ok;
       asm volatile("cp.async.wait_group 0;" ::: "memory"); // no copy outlives the CTA
     }
   } else if (warp < 12) {
@@ -253,26 +261,79 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         if (lane == 0) mbarArrive(pReady + 16 * chain + 8 * half);
       });
     }
-    if (ok && mine > 0 && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * chain, 0, abortP, 3))) ok = false;
-    if (ok && !padding) {
-      tcFenceAfter();
-      const bool live = row < draft * p.G;
-      const int64_t part = (((static_cast<int64_t>(b) * p.nq + row / p.G) * p.heads + kvh * p.G + row % p.G) * p.splits + split) * 2 + chain;
+    // All products are done (the ring is free) before the odd chain leaves its output there, one column per row.
+    for (int c = 0; c < 2; ++c) {
+      if (ok && tiles > c && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * c, 0, abortP, 3))) ok = false;
+    }
+    tcFenceAfter();
+    const uint32_t slot = sRing + lrow * 4; // [dim][row], then maxima, sums
+    if (ok && chain == 1 && tiles > 1) {
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
-        if (mine > 0) {
+        tcLoad32(oAddr + c * 32, r);
+        tcWaitLd();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + (c * 32 + i) * 512), "r"(r[i]) : "memory");
+      }
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + D * 512), "f"(ref) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + (D + 1) * 512), "f"(l) : "memory");
+      __syncwarp();
+      if (lane == 0) mbarArrive(handed);
+    }
+    if (ok && chain == 0 && !padding) {
+      float f0 = 1.0f, f1 = 0.0f;
+      if (tiles > 1) {
+        if (!__all_sync(0xffffffffu, mbarWait(handed, 0, abortP, 7))) ok = false;
+        float ref1, l1;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=f"(ref1) : "r"(slot + D * 512));
+        asm volatile("ld.shared.b32 %0, [%1];" : "=f"(l1) : "r"(slot + (D + 1) * 512));
+        const float both = fmaxf(ref, ref1);
+        f0 = ref == -INFINITY ? 0.0f : fastExp2((ref - both) * sl2);
+        f1 = ref1 == -INFINITY ? 0.0f : fastExp2((ref1 - both) * sl2);
+        l = l * f0 + l1 * f1;
+        ref = both;
+      }
+      const bool live = ok && row < draft * p.G;
+      const int64_t orow = (static_cast<int64_t>(b) * p.nq + row / p.G) * p.heads + kvh * p.G + row % p.G, part = orow * p.splits + split;
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (tiles > 0) {
           tcLoad32(oAddr + c * 32, r);
           tcWaitLd();
-          if (live) {
+        }
+        if (!live) continue;
+        float x[32];
 #pragma unroll
-            for (int g = 0; g < 8; ++g)
-              *reinterpret_cast<uint4 *>(p.po + part * D + c * 32 + g * 4) = make_uint4(r[g * 4], r[g * 4 + 1], r[g * 4 + 2], r[g * 4 + 3]);
+        for (int i = 0; i < 32; ++i) {
+          x[i] = tiles > 0 && f0 != 0.0f ? __uint_as_float(r[i]) * f0 : 0.0f; // a chain that saw nothing of the row does not count
+          if (f1 != 0.0f) {
+            float o1;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=f"(o1) : "r"(slot + (c * 32 + i) * 512));
+            x[i] = fmaf(o1, f1, x[i]);
+          }
+        }
+        if (p.splits > 1) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) *reinterpret_cast<float4 *>(p.po + part * D + c * 32 + g * 4) = make_float4(x[g * 4], x[g * 4 + 1], x[g * 4 + 2], x[g * 4 + 3]);
+        } else {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (l > 0.0f) {
+              w.x = packPair<T>(x[g * 8] * inv, x[g * 8 + 1] * inv);
+              w.y = packPair<T>(x[g * 8 + 2] * inv, x[g * 8 + 3] * inv);
+              w.z = packPair<T>(x[g * 8 + 4] * inv, x[g * 8 + 5] * inv);
+              w.w = packPair<T>(x[g * 8 + 6] * inv, x[g * 8 + 7] * inv);
+            }
+            *reinterpret_cast<uint4 *>(out + orow * D + c * 32 + g * 8) = w;
           }
         }
       }
-      if (live) {
-        p.pm[part] = ref == -INFINITY ? -INFINITY : ref * sl2; // an empty part is skipped by the join, whatever its output holds
+      if (live && p.splits > 1) {
+        p.pm[part] = ref == -INFINITY ? -INFINITY : ref * sl2;
         p.pl[part] = l;
       }
     }
@@ -284,12 +345,13 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
       auto desc = [](uint32_t low) -> uint64_t { return (static_cast<uint64_t>(HIGH) << 32) | low; };
       const uint32_t qLow = sQ >> 4;
       bool ok = mbarWait(qFull, 0, abortP, 4);
-      int stage = 0, phase = 0, old = 0; // stage of tile j, of tile j - 2
+      int stage = 0, phase = 0, old = 0, oldPhase = 0; // of tile j, of tile j - 2
       for (int j = 0; ok && j < tiles + 2; ++j) {
         const int chain = j & 1;
         const uint32_t sCol = tmemBase + chain * 128, oCol = tmemBase + 256 + chain * D;
         if (j >= 2) { // O += P V of the chain's tile before
           const uint32_t vLow = ((sRing + (2 * old + 1) * TILE) >> 4) | (static_cast<uint32_t>(COLS >> 4) << 16);
+          ok = mbarWait(full + 8 * (R + old), oldPhase, abortP, 8);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             ok = ok && mbarWait(pReady + 16 * chain + 8 * h, ((j - 2) >> 1) & 1, abortP, 5);
@@ -300,9 +362,12 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
             }
           }
           if (!ok) break;
-          tcCommit(empty + 8 * old);
+          tcCommit(empty + 8 * (R + old));
           if (j + 2 > tiles + 1) tcCommit(oFull + 8 * chain); // the chain's last tile
-          old = old == R - 1 ? 0 : old + 1;
+          if (++old == R) {
+            old = 0;
+            oldPhase ^= 1;
+          }
         }
         if (j < tiles) {
           ok = mbarWait(full + 8 * stage, phase, abortP, 6);
@@ -315,6 +380,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
             tcMma(sCol, desc(qLow + off), desc(kLow + off), idS, ks > 0);
           }
           tcCommit(sFull + 8 * chain);
+          tcCommit(empty + 8 * stage);
           if (++stage == R) {
             stage = 0;
             phase ^= 1;
@@ -333,7 +399,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
 }
 
 template <typename T, int D>
-static int launchCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, int batch, AcParams p, cudaStream_t st) {
+static int launchCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, void *out, int batch, AcParams p, cudaStream_t st) {
   // The cache as [blocks, kv heads, block size, D] in boxes of 32 rows; without one every row is copied on its own.
   CUtensorMap mapK = {}, mapV = {};
   const int64_t extents[4] = {D, p.blockSize, p.kvHeads, p.blocks}, row = D, head = row * p.blockSize, strides[3] = {row, head, head * p.kvHeads};
@@ -350,20 +416,21 @@ static int launchCachedTcgen05(const void *q, const void *k, const void *v, cons
   TTB_CHECK(mts * p.splits <= 0x7fffffff, "too many query rows");
   dim3 grid(static_cast<unsigned>(mts * p.splits), static_cast<unsigned>(p.kvHeads), static_cast<unsigned>(batch));
   TTB_CUDA(launchPdl(sdpaCachedTcgen05Kernel<T, D>, grid, dim3(AC_THREADS), AcShape<D>::SMEM, st, mapK, mapV,
-                     static_cast<const T *>(q), static_cast<const T *>(k), static_cast<const T *>(v), static_cast<const T *>(kd), static_cast<const T *>(vd), p));
+                     static_cast<const T *>(q), static_cast<const T *>(k), static_cast<const T *>(v), static_cast<const T *>(kd), static_cast<const T *>(vd),
+                     static_cast<T *>(out), p));
   countLaunch();
   TTB_LAUNCH_CHECK();
   return TTB_OK;
 }
 
-// The tree's rows over p.splits runs of slots, two partial results each; the caller joins them.  16-bit types, head_dim
-// 64 or 128, a positive scale.
-int sdpaCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, int dtype, int dim, int batch, const AcParams &p,
+// The tree's rows over p.splits runs of slots: the result itself, or with several runs the partial results of each, which
+// the caller joins.  16-bit types, head_dim 64 or 128, a positive scale.
+int sdpaCachedTcgen05(const void *q, const void *k, const void *v, const void *kd, const void *vd, void *out, int dtype, int dim, int batch, const AcParams &p,
                       cudaStream_t st) {
   if (dtype == kBF16) {
-    return dim == 64 ? launchCachedTcgen05<__nv_bfloat16, 64>(q, k, v, kd, vd, batch, p, st) : launchCachedTcgen05<__nv_bfloat16, 128>(q, k, v, kd, vd, batch, p, st);
+    return dim == 64 ? launchCachedTcgen05<__nv_bfloat16, 64>(q, k, v, kd, vd, out, batch, p, st) : launchCachedTcgen05<__nv_bfloat16, 128>(q, k, v, kd, vd, out, batch, p, st);
   }
-  return dim == 64 ? launchCachedTcgen05<__half, 64>(q, k, v, kd, vd, batch, p, st) : launchCachedTcgen05<__half, 128>(q, k, v, kd, vd, batch, p, st);
+  return dim == 64 ? launchCachedTcgen05<__half, 64>(q, k, v, kd, vd, out, batch, p, st) : launchCachedTcgen05<__half, 128>(q, k, v, kd, vd, out, batch, p, st);
 }
 
 } // namespace ttb

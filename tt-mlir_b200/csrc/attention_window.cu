@@ -533,15 +533,14 @@ static int windowSplits(int64_t batch, int64_t kvHeads, int64_t rows, int64_t ma
 // How a tree's rows are computed, from the sizes that its workspace is asked for with.
 struct TreePlan {
   bool tall;  // tensor-core kernel with 128-row tiles
-  int splits; // runs of slots per row tile
-  int parts;  // partial results per row (1: none, the result itself)
+  int splits; // runs of slots per row tile, a partial result each (1: the result itself)
 };
 static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kvHeads, int64_t dim, int64_t positions) {
   const int64_t rows = nodes * (heads / kvHeads), slots = positions + nodes;
   TreePlan t;
   t.tall = rows > 32 && (dim == 64 || dim == 128);
   if (!t.tall) {
-    t.parts = t.splits = windowSplits(batch, kvHeads, rows, slots);
+    t.splits = windowSplits(batch, kvHeads, rows, slots);
     return t;
   }
   // One CTA per SM: waves x (tiles per CTA + 6 for what a CTA costs besides), at the longest possible length.
@@ -555,7 +554,6 @@ static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kv
       t.splits = static_cast<int>(s);
     }
   }
-  t.parts = 2 * t.splits;
   return t;
 }
 
@@ -780,7 +778,7 @@ int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const vo
 
 size_t ttb_sdpa_tree_workspace_bytes(int batch, int nodes, int heads, int kv_heads, int head_dim, int64_t positions) {
   if (batch <= 0 || nodes <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || positions <= 0 || heads % kv_heads) return 0;
-  return windowPartBytes(batch, nodes, heads, head_dim, treePlan(batch, nodes, heads, kv_heads, head_dim, positions).parts);
+  return windowPartBytes(batch, nodes, heads, head_dim, treePlan(batch, nodes, heads, kv_heads, head_dim, positions).splits);
 }
 
 int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const void *k_cache, const void *v_cache, const void *page_table,
@@ -809,7 +807,7 @@ int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const
   p.qh = p.oh = head_dim;
   // The workspace must not depend on the window (its size is asked for without one), so neither do the splits.
   const TreePlan plan = treePlan(batch, nodes, heads, kv_heads, head_dim, positions);
-  p.splits = plan.parts;
+  p.splits = plan.splits;
   const size_t need = windowPartBytes(batch, nodes, heads, head_dim, p.splits);
   TTB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (see ttb_sdpa_tree_workspace_bytes)");
   const int flagged = indexBadFlag(&p.bad);
@@ -831,8 +829,8 @@ int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const
     a.fmt = dtype == kBF16 ? 1 : 0;
     a.scaleLog2 = p.scaleLog2;
     a.pm = p.pm; a.pl = p.pl; a.po = p.po;
-    const int rc2 = sdpaCachedTcgen05(q, k_cache, v_cache, k_draft, v_draft, dtype, head_dim, batch, a, st);
-    if (rc2) return rc2;
+    const int rc2 = sdpaCachedTcgen05(q, k_cache, v_cache, k_draft, v_draft, out, dtype, head_dim, batch, a, st);
+    if (rc2 || p.splits == 1) return rc2;
     if (dtype == kBF16) return head_dim == 64 ? launchWindowJoin<__nv_bfloat16, 64>(out, p, st) : launchWindowJoin<__nv_bfloat16, 128>(out, p, st);
     return head_dim == 64 ? launchWindowJoin<__half, 64>(out, p, st) : launchWindowJoin<__half, 128>(out, p, st);
   }
