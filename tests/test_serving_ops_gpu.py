@@ -175,9 +175,9 @@ TREES = [  # dtype, heads, kv heads, dim, block, cached tokens, nodes, kind, win
 
 
 @pytest.mark.parametrize("dtype,H,Hkv,D,block,lens,T,kind,window,sinks,drafts,shared", TREES)
-def test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared):
+def test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared, room=0):
     gen = torch.Generator().manual_seed(T * 31 + D)
-    B, N = len(lens), max(max(lens), 1)
+    B, N = len(lens), max(max(lens), 1, room)
     q, kd, vd = rand(gen, B, T, H, D, dtype=dtype), rand(gen, B, T, Hkv, D, dtype=dtype), rand(gen, B, T, Hkv, D, dtype=dtype)
     dk, dv = rand(gen, B, Hkv, N, D, dtype=dtype), rand(gen, B, Hkv, N, D, dtype=dtype)
     k, v, table = paged(gen, dk, dv, block, lens, dtype)
@@ -206,6 +206,19 @@ def test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts,
         want, tol = attend(q[b, :t].transpose(0, 1), keys, vals, torch.cat([cached, fresh], dim=1), 1 / math.sqrt(D), dtype)
         check(got[b, :t].transpose(0, 1), want, tol, f"user {b}")
     assert kn.bad() == 0
+
+
+@pytest.mark.parametrize("dtype,H,Hkv,D,block,lens,T,kind,window,sinks,drafts,shared", [
+    (torch.bfloat16, 8, 2, 128, 32, [100, 0, 1, 2300], 1, "star", 0, 0, None, False),
+    (torch.float16, 4, 4, 64, 24, [333, 5, 2200], 13, "random", 50, 4, [13, 6, 0], False),
+    (torch.bfloat16, 16, 2, 128, 64, [700, 129, 2304], 64, "random", 0, 0, [64, 63, 1], True),
+    (torch.bfloat16, 3, 1, 128, 7, [90, 2200], 17, "chain", 12, 3, None, True),
+    (torch.float16, 5, 1, 64, 100, [1000], 64, "chain", 30, 1010, None, False),
+    (torch.bfloat16, 32, 4, 128, 64, [2303, 513], 33, "star", 100, 0, None, False),
+    (torch.bfloat16, 8, 8, 64, 128, [2048, 127, 128], 5, "random", 1500, 33, None, False),
+    (torch.float16, 8, 1, 128, 40, [2280], 40, "random", 10 ** 12, 2, [33], False)])
+def test_tree_in_a_large_cache(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared):
+    test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared, room=2304)
 
 
 def test_tree_reports_a_parent_that_is_not_an_earlier_node(kn):

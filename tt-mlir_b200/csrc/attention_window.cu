@@ -532,13 +532,16 @@ static int windowSplits(int64_t batch, int64_t kvHeads, int64_t rows, int64_t ma
 
 // How a tree's rows are computed, from the sizes that its workspace is asked for with.
 struct TreePlan {
-  bool tall;  // tensor-core kernel with 128-row tiles
+  bool tall;  // tensor-core kernel with tiles of 128 rows and 128 slots
   int splits; // runs of slots per row tile, a partial result each (1: the result itself)
 };
 static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kvHeads, int64_t dim, int64_t positions) {
   const int64_t rows = nodes * (heads / kvHeads), slots = positions + nodes;
   TreePlan t;
-  t.tall = rows > 32 && (dim == 64 || dim == 128);
+  // The tensor-core kernel reads faster but starts slower (128 KB of ring to fill, tensor memory to claim).  Measured with
+  // 8 kv heads x 4, head_dim 128, this kernel / that one, us: 1 user, 1000 tokens, 4 .. 32 nodes: 19 .. 26 / 27 .. 32;
+  // 4 users, 4000 tokens, 8 nodes: 42 / 36; 16 users, 8192 tokens, 4 nodes: 120 / 107, 16 nodes: 177 / 109.
+  t.tall = slots >= 2048 && (dim == 64 || dim == 128);
   if (!t.tall) {
     t.splits = windowSplits(batch, kvHeads, rows, slots);
     return t;
