@@ -261,7 +261,8 @@ class OracleBuilder:
     def update_cache(self, cache, x, update_index, batch_offset=0, loc=None):
         return _map(lambda c, t, i: ops.update_cache(c, t, i, batch_offset), cache, x, update_index)
 
-    def scaled_dot_product_attention_decode(self, q, k, v, cur_pos=None, mask=None, is_causal=True, scale=None, loc=None):
+    def scaled_dot_product_attention_decode(self, q, k, v, cur_pos=None, mask=None, is_causal=True, scale=None,
+                                            sliding_window_size=None, loc=None):
         vals = [x for x in (q, k, v, cur_pos, mask) if x is not None]
 
         def fn(*ts):
@@ -269,7 +270,7 @@ class OracleBuilder:
             qq, kk, vv = next(it), next(it), next(it)
             cp = next(it) if cur_pos is not None else None
             mk = next(it) if mask is not None else None
-            return ops.sdpa_decode(qq, kk, vv, cp, mk, is_causal, scale)
+            return ops.sdpa_decode(qq, kk, vv, cp, mk, is_causal, scale, sliding_window_size)
         return _map(fn, *vals)
 
     def paged_update_cache(self, cache, x, update_index, page_table=None, share_cache=False, loc=None):
@@ -283,7 +284,7 @@ class OracleBuilder:
         return _map(lambda c, t, pt, bi: ops.paged_fill_cache(c, t, pt, bi), cache, x, page_table, batch_idx)
 
     def paged_scaled_dot_product_attention_decode(self, q, k, v, page_table, cur_pos=None, mask=None, is_causal=True, scale=None,
-                                                  loc=None):
+                                                  sliding_window_size=None, loc=None):
         vals = [x for x in (q, k, v, page_table, cur_pos, mask) if x is not None]
 
         def fn(*ts):
@@ -291,7 +292,7 @@ class OracleBuilder:
             qq, kk, vv, pt = next(it), next(it), next(it), next(it)
             cp = next(it) if cur_pos is not None else None
             mk = next(it) if mask is not None else None
-            return ops.paged_sdpa_decode(qq, kk, vv, pt, cp, is_causal, scale, mk)
+            return ops.paged_sdpa_decode(qq, kk, vv, pt, cp, is_causal, scale, mk, sliding_window_size)
         return _map(fn, *vals)
 
     def gather(self, x, index, dim, loc=None): return _map(lambda t, i: ops.gather(t, i, dim), x, index)
@@ -346,9 +347,9 @@ class OracleBuilder:
 
     def rotary_embedding(self, x, cos, sin, loc=None): return _map(ops.rotary_embedding, x, cos, sin)
 
-    def scaled_dot_product_attention(self, q, k, v, is_causal=True, mask=None, scale=None, loc=None):
+    def scaled_dot_product_attention(self, q, k, v, is_causal=True, mask=None, scale=None, sliding_window_size=None, loc=None):
         if mask is None:
-            return _map(lambda a, b, c: ops.sdpa(a, b, c, is_causal, None, scale), q, k, v)
+            return _map(lambda a, b, c: ops.sdpa(a, b, c, is_causal, None, scale, sliding_window_size), q, k, v)
         return _map(lambda a, b, c, m: ops.sdpa(a, b, c, is_causal, m, scale), q, k, v, mask)
 
     # ---- mesh

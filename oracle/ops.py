@@ -402,9 +402,10 @@ def update_cache(cache, x, update_index, batch_offset=0):
     return out
 
 
-def sdpa_decode(q, k, v, cur_pos=None, mask=None, is_causal=True, scale=None):
+def sdpa_decode(q, k, v, cur_pos=None, mask=None, is_causal=True, scale=None, window=None):
     """mapping.py:2417-2482 (sdpa_decode_golden): q [1, B, H, D], k / v [B, Hkv, S, D]; the mask
-    [B|1, 1, H|1, S] is added before the scale; causal = keys after cur_pos[b] are -inf."""
+    [B|1, 1, H|1, S] is added before the scale; causal = keys after cur_pos[b] are -inf.  `window` (the op's
+    sliding_window_size): keys up to cur_pos[b] - window are -inf too."""
     qq = q.float().squeeze(0).unsqueeze(2)                      # [B, H, 1, D]
     kk, vv = k.float(), v.float()
     rep = qq.shape[1] // kk.shape[1]
@@ -418,6 +419,8 @@ def sdpa_decode(q, k, v, cur_pos=None, mask=None, is_causal=True, scale=None):
         cm = torch.zeros((qk.shape[0], 1, 1, qk.shape[3]), dtype=torch.float32)
         for i in range(qk.shape[0]):
             cm[i, :, :, int(cur_pos[i].item()) + 1:] = float("-inf")
+            if window:
+                cm[i, :, :, :max(0, int(cur_pos[i].item()) + 1 - window)] = float("-inf")
         qk = qk + cm
     if scale is not None:
         qk = qk * scale
@@ -458,7 +461,8 @@ def rotary_embedding(x, cos, sin):
     return _hoist(fn, x.dtype, x, cos, sin)
 
 
-def sdpa(q, k, v, is_causal=True, mask=None, scale=None):  # mapping.py:8398-8500
+def sdpa(q, k, v, is_causal=True, mask=None, scale=None, window=None):  # mapping.py:8398-8500
+    # window (the op's sliding_window_size): with the causal mask, keys j <= i - window are masked too
     hq, hkv = q.shape[1], k.shape[1]
     if hq != hkv:
         k = torch.repeat_interleave(k, hq // hkv, dim=1)
@@ -470,6 +474,8 @@ def sdpa(q, k, v, is_causal=True, mask=None, scale=None):  # mapping.py:8398-850
     if is_causal and mask is None:
         sq, sk = qk.shape[-2], qk.shape[-1]
         qk = torch.add(qk, torch.triu(torch.full((sq, sk), float("-inf")), diagonal=1))
+        if window:
+            qk = torch.add(qk, torch.tril(torch.full((sq, sk), float("-inf")), diagonal=-window))
     if mask is not None:
         qk = torch.add(qk, mask.float())
     w = torch.softmax(qk, dim=-1)
@@ -580,9 +586,10 @@ def paged_fill_cache(cache, x, page_table, batch_idx=None):
     return out
 
 
-def paged_sdpa_decode(q, k_cache, v_cache, page_table, cur_pos=None, is_causal=True, scale=None, mask=None):
+def paged_sdpa_decode(q, k_cache, v_cache, page_table, cur_pos=None, is_causal=True, scale=None, mask=None, window=None):
     """ttir_paged_sdpa_decode_golden: q [B, 1, H, D]; caches [blocks, Hkv, block_size, D]; keys after
-    cur_pos[b] get the most negative f32 (pre-scaled, as the golden has it) and the softmax runs in f32."""
+    cur_pos[b] get the most negative f32 (pre-scaled, as the golden has it) and the softmax runs in f32.
+    `window` (the op's sliding_window_size): so do the keys up to cur_pos[b] - window."""
     b, sq, h, d = q.shape
     blocks, hkv, block_size, _ = k_cache.shape
     per_user = page_table.shape[-1]
@@ -603,6 +610,8 @@ def paged_sdpa_decode(q, k_cache, v_cache, page_table, cur_pos=None, is_causal=T
         m = torch.zeros((b, h, sq, seq), dtype=torch.float32)
         for i in range(b):
             m[i, :, :, int(cur_pos[i].item()) + 1:] = torch.finfo(torch.float32).min
+            if window:
+                m[i, :, :, :max(0, int(cur_pos[i].item()) + 1 - window)] = torch.finfo(torch.float32).min
     if m is not None:
         m = m * (scale if scale is not None else d ** -0.5)
     o = F.scaled_dot_product_attention(q.float().permute(0, 2, 1, 3), kk, vv, attn_mask=m, scale=scale, is_causal=False)

@@ -951,6 +951,8 @@ private:
   void runPad(const fbt::PadOp *op);
   void runFillCache(const fbt::FillCacheOp *op);
   void runUpdateCache(const fbt::UpdateCacheOp *op);
+  void runWindowDecode(const TensorPtr &q, const TensorPtr &k, const TensorPtr &v, const TensorPtr &table, const TensorPtr &pos, const TensorPtr &out,
+                       int B, int H, int Hkv, int blocks, int blockSize, int pages, int D, uint32_t window, float scale);
   void runSdpaDecode(const fbt::ScaledDotProductAttentionDecodeOp *op);
   // sub-programs: const-eval cache, calls, traces
   std::vector<TensorPtr> runSubProgram(uint32_t index, const std::vector<TensorPtr> &inputs);
@@ -4123,10 +4125,21 @@ void Executor::runUpdateCache(const fbt::UpdateCacheOp *op) {
   root->version.store(TensorImpl::nextTensorVersion());
 }
 
+// One token per user inside a sliding window over a dense (table null) or paged cache.
+void Executor::runWindowDecode(const TensorPtr &q, const TensorPtr &k, const TensorPtr &v, const TensorPtr &table, const TensorPtr &pos,
+                               const TensorPtr &out, int B, int H, int Hkv, int blocks, int blockSize, int pages, int D, uint32_t window, float scale) {
+  const size_t wsBytes = ttb_sdpa_window_decode_workspace_bytes(B, H, Hkv, D, static_cast<int64_t>(pages) * blockSize, window, 0);
+  TensorPtr ws = wsBytes ? makeDeviceTensor(dev, {static_cast<uint32_t>((wsBytes + 3) / 4)}, DataType::Float32) : nullptr;
+  eachRank([&](size_t i, const RankCtx &r) {
+    TTB_CALL(ttb_sdpa_window_decode(q->shards[i]->ptr, k->shards[i]->ptr, v->shards[i]->ptr, table ? table->shards[i]->ptr : nullptr,
+                                    pos->shards[i]->ptr, out->shards[i]->ptr, ttbDtype(q->dtype), B, H, Hkv, blocks, blockSize, pages, D, window, 0,
+                                    scale, ws ? ws->shards[i]->ptr : nullptr, wsBytes, r.stream));
+  });
+}
+
 // q [1, B, H, D] against k, v [B, Hkv, S, D] (the decode layout, tools/golden/mapping.py:2431-2437).
 void Executor::runSdpaDecode(const fbt::ScaledDotProductAttentionDecodeOp *op) {
   TTRT_ASSERT(!op->attention_sink(), "attention sinks are not supported");
-  TTRT_ASSERT(!op->sliding_window_size().has_value(), "sliding-window decode attention is not supported");
   TensorPtr q = getDevice(op->query()), k = getDevice(op->key()), v = getDevice(op->value());
   TensorPtr mask = op->attention_mask() ? getDevice(op->attention_mask()) : nullptr;
   TensorPtr pos = op->cur_pos_tensor() ? getDevice(op->cur_pos_tensor()) : nullptr;
@@ -4150,6 +4163,12 @@ void Executor::runSdpaDecode(const fbt::ScaledDotProductAttentionDecodeOp *op) {
   }
   // The golden applies no scaling when the op carries none (tools/golden/mapping.py:2471-2473).
   const float scale = op->scale().has_value() ? *op->scale() : 1.0f;
+  if (op->sliding_window_size().has_value()) {
+    TTRT_ASSERT(op->is_causal() && pos && !mask, "a sliding window needs positions and no mask");
+    runWindowDecode(q, k, v, nullptr, pos, out, B, H, Hkv, B, S, 1, D, *op->sliding_window_size(), scale);
+    put(op->out(), out);
+    return;
+  }
   const size_t wsBytes = ttb_sdpa_decode_workspace_bytes(B, H, S, D);
   std::vector<uint32_t> wsShape{static_cast<uint32_t>((wsBytes + 3) / 4)};
   TensorPtr ws = makeDeviceTensor(dev, wsShape, DataType::Float32);
@@ -4209,7 +4228,6 @@ void Executor::runPagedFillCache(const fbt::PagedFillCacheOp *op) {
 // q [B, 1, H, D] against paged k, v [blocks, Hkv, block_size, D] (tools/golden/mapping.py:8745-8844).
 void Executor::runPagedSdpaDecode(const fbt::PagedScaledDotProductAttentionDecodeOp *op) {
   TTRT_ASSERT(!op->attention_sink(), "attention sinks are not supported");
-  TTRT_ASSERT(!op->sliding_window_size().has_value(), "sliding-window decode attention is not supported");
   TensorPtr q = getDevice(op->query()), k = getDevice(op->key()), v = getDevice(op->value());
   TensorPtr table = castOnDevice(getDevice(op->page_table()), DataType::Int32);
   TensorPtr mask = op->attention_mask() ? getDevice(op->attention_mask()) : nullptr;
@@ -4237,6 +4255,12 @@ void Executor::runPagedSdpaDecode(const fbt::PagedScaledDotProductAttentionDecod
   }
   // torch's scaled_dot_product_attention, which the golden calls, scales by 1 / sqrt(D) when no scale is given
   const float scale = op->scale().has_value() ? *op->scale() : 1.0f / std::sqrt(static_cast<float>(D));
+  if (op->sliding_window_size().has_value()) {
+    TTRT_ASSERT(op->is_causal() && pos && !mask, "a sliding window needs positions and no mask");
+    runWindowDecode(q, k, v, table, pos, out, B, H, Hkv, blocks, blockSize, pages, D, *op->sliding_window_size(), scale);
+    put(op->out(), out);
+    return;
+  }
   const size_t wsBytes = ttb_sdpa_decode_workspace_bytes(B, H, S, D);
   TensorPtr ws = makeDeviceTensor(dev, {static_cast<uint32_t>((wsBytes + 3) / 4)}, DataType::Float32);
   eachRank([&](size_t i, const RankCtx &r) {
@@ -4683,7 +4707,7 @@ void Executor::runSdpa(const fbt::ScaledDotProductAttentionOp *op) {
   TensorPtr q = getDevice(op->query()), k = getDevice(op->key()), v = getDevice(op->value());
   TensorPtr mask = op->attention_mask() ? getDevice(op->attention_mask()) : nullptr;
   TTRT_ASSERT(!op->attention_sink(), "attention_sink is not supported");
-  TTRT_ASSERT(!op->sliding_window_size().has_value(), "sliding_window_size is not supported");
+  TTRT_ASSERT(!op->sliding_window_size().has_value() || (op->is_causal() && !mask), "a sliding window needs the causal mask and no other");
   TensorPtr out = allocOut(op->out());
   TTRT_ASSERT(q->shape.size() == 4 && k->shape.size() == 4 && v->shape.size() == 4, "attention operands must be [batch, heads, seq, head_dim]");
   int64_t B = q->shape[0], Hq = q->shape[1], Sq = q->shape[2], D = q->shape[3];
@@ -4700,6 +4724,11 @@ void Executor::runSdpa(const fbt::ScaledDotProductAttentionOp *op) {
     mh = mask->shape[1];
   }
   eachRank([&](size_t i, const RankCtx &r) {
+    if (op->sliding_window_size().has_value()) {
+      TTB_CALL(ttb_sdpa_window(q->shards[i]->ptr, k->shards[i]->ptr, v->shards[i]->ptr, nullptr, out->shards[i]->ptr, ttbDtype(q->dtype), B, Hq, Hkv,
+                               Sq, Skv, D, nullptr, nullptr, nullptr, nullptr, 0, *op->sliding_window_size(), 0, scale, r.stream));
+      return;
+    }
     TTB_CALL(ttb_sdpa(q->shards[i]->ptr, k->shards[i]->ptr, v->shards[i]->ptr, mask ? mask->shards[i]->ptr : nullptr,
                       out->shards[i]->ptr, ttbDtype(q->dtype), B, Hq, Hkv, Sq, Skv, D, mb, mh, op->is_causal() ? 1 : 0, scale,
                       r.stream));

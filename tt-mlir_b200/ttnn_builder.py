@@ -448,11 +448,13 @@ class ProgramBuilder:
         return out
 
     def scaled_dot_product_attention(self, q: Value, k: Value, v: Value, is_causal: bool = True,
-                                     mask: Optional[Value] = None, scale: Optional[float] = None, loc=None) -> Value:
+                                     mask: Optional[Value] = None, scale: Optional[float] = None,
+                                     sliding_window_size: Optional[int] = None, loc=None) -> Value:
         out = self._value(q.shape, q.dtype)
         self._emit("ScaledDotProductAttentionOp", {
             "query": q.ref, "key": k.ref, "value": v.ref, "is_causal": is_causal,
-            "attention_mask": mask.ref if mask else None, "scale": scale, "out": out.ref, "memcfg": self._mc()},
+            "attention_mask": mask.ref if mask else None, "scale": scale, "sliding_window_size": sliding_window_size,
+            "out": out.ref, "memcfg": self._mc()},
             [q, k, v] + ([mask] if mask else []), [out], loc)
         return out
 
@@ -1139,13 +1141,14 @@ class ProgramBuilder:
 
     def scaled_dot_product_attention_decode(self, q: Value, k: Value, v: Value, cur_pos: Optional[Value] = None,
                                             mask: Optional[Value] = None, is_causal: bool = True,
-                                            scale: Optional[float] = None, loc=None) -> Value:
+                                            scale: Optional[float] = None, sliding_window_size: Optional[int] = None,
+                                            loc=None) -> Value:
         out = self._value(q.shape, q.dtype)
         ins = [x for x in (q, k, v, mask, cur_pos) if x is not None]
         self._emit("ScaledDotProductAttentionDecodeOp", {
             "query": q.ref, "key": k.ref, "value": v.ref, "is_causal": is_causal,
             "attention_mask": mask.ref if mask else None, "cur_pos_tensor": cur_pos.ref if cur_pos else None,
-            "scale": scale, "out": out.ref, "memcfg": self._mc()}, ins, [out], loc)
+            "scale": scale, "sliding_window_size": sliding_window_size, "out": out.ref, "memcfg": self._mc()}, ins, [out], loc)
         return out
 
     def paged_update_cache(self, cache: Value, x: Value, update_index: Value, page_table: Optional[Value] = None,
@@ -1167,14 +1170,15 @@ class ProgramBuilder:
 
     def paged_scaled_dot_product_attention_decode(self, q: Value, k: Value, v: Value, page_table: Value,
                                                   cur_pos: Optional[Value] = None, mask: Optional[Value] = None,
-                                                  is_causal: bool = True, scale: Optional[float] = None, loc=None) -> Value:
+                                                  is_causal: bool = True, scale: Optional[float] = None,
+                                                  sliding_window_size: Optional[int] = None, loc=None) -> Value:
         """q [B, 1, H, D] against paged k / v [blocks, Hkv, block_size, D] read through page_table [B, pages]."""
         out = self._value(q.shape, q.dtype)
         ins = [x for x in (q, k, v, page_table, mask, cur_pos) if x is not None]
         self._emit("PagedScaledDotProductAttentionDecodeOp", {
             "query": q.ref, "key": k.ref, "value": v.ref, "page_table": page_table.ref, "is_causal": is_causal,
             "attention_mask": mask.ref if mask else None, "cur_pos_tensor": cur_pos.ref if cur_pos else None,
-            "scale": scale, "out": out.ref, "memcfg": self._mc()}, ins, [out], loc)
+            "scale": scale, "sliding_window_size": sliding_window_size, "out": out.ref, "memcfg": self._mc()}, ins, [out], loc)
         return out
 
     # ---- indexing ---------------------------------------------------------------------------------------------------
