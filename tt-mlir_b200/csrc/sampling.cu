@@ -17,8 +17,8 @@
 //    the border and the next interval is chosen inside the bracket, so the search always ends.  The first interval is
 //    open above and sized for some 2500 entries, which answers most top-k and top-p settings at once and finds the
 //    largest logit on the way.
-//  * The draw is a search too: the 16 warps weigh 16 consecutive runs, the run that holds u times the total is split
-//    among the 16 warps again, until 32 entries are left.
+//  * The draw is a search too: of the warps' runs the one that holds u times the total, of it the thread's part that
+//    does, until 32 entries are left.  After a cut the last pass knows the runs' weights already.
 // What bounds it: instruction issue, at some 10 instructions per entry and pass.
 #include "common.cuh"
 
@@ -29,10 +29,10 @@ namespace ttb {
 constexpr int SL_THREADS = 512;
 constexpr int SL_WARPS = SL_THREADS / 32;
 constexpr int SL_KEEP = 23;                 // entries a thread can collect in one pass
-constexpr int SL_LIST = 4096;               // entries that fit: 8 per thread on average, 24 once in 10^6 threads
+constexpr int SL_LIST = 5120;               // entries that fit: 10 per thread on average, 24 at any of them once in 40 rows
 constexpr int SL_SHORT = 8192;              // rows up to this length fit whole: 16 entries per thread, and one of the ragged ends
 constexpr int SL_SAMPLE = 4096;
-constexpr int SL_STAGES = 6;                // 16-byte vectors of a thread in flight, and the one at work
+constexpr int SL_STAGES = 6;                // 16-byte vectors of a thread in flight
 constexpr int SL_BINS = 1024;               // two per thread
 constexpr float SL_FIRST = 2500.0f;         // entries aimed at by the first pass
 constexpr float SL_FLOOR = 60.0f;           // octaves below the largest weight that count
@@ -41,13 +41,16 @@ constexpr int SL_HALF = 18;                 // ... of 18 bits each, whose sums s
 constexpr int64_t SL_MAX_VOCAB = 1 << 22;
 static_assert(SL_BINS == 2 * SL_THREADS && SL_THREADS * SL_KEEP < 1 << 14, "bins per thread; the halves' sums fit 32 bits");
 
-// What one pass found: entries at and above lo and hi, weight at and above lo and another bound, the largest logit.
+// What one pass found: entries and weight at and above lo and hi, the weight at and above a third bound and of everything,
+// the largest logit.
 struct PassResult {
-  double mLo, mFrom;
+  double mLo, mHi, mHigh, mAll;
   unsigned int cLo, cHi;
   float top;
   bool fits; // no thread collected more than it can keep
 };
+
+enum { KNOWN_NOTHING, KNOWN_LIST, KNOWN_TOP };
 
 struct alignas(16) SampleSmem {
   union {
@@ -58,7 +61,7 @@ struct alignas(16) SampleSmem {
   };
   float list[SL_KEEP][SL_THREADS]; // column t: what thread t collected
   float sample[SL_SAMPLE];
-  double dRed[2][SL_WARPS];
+  double dRed[4][SL_WARPS];
   unsigned long long uRed[2][SL_WARPS], picked, rest;
   float fRed[2][SL_WARPS];
   unsigned int cRed[2][SL_WARPS];
@@ -68,10 +71,12 @@ struct alignas(16) SampleSmem {
   // the draw's current run and target
   int from, to, ok;
   double target, total;
-  unsigned long long equalBefore;
+  unsigned int equalBefore;
   // results of the search's steps, written by one thread and read by all
   PassResult pass;
-  float border, lo, hi;
+  double runAbove[SL_WARPS]; // per warp's run: the weight at and above hi
+  float runTop[SL_WARPS];    // ... and the largest logit
+  float border, lo, hi, high;
   unsigned int ties;
   unsigned long long through;
 };
@@ -119,12 +124,12 @@ struct Weigher {
 };
 
 // Calls f(v) for entries lo .. hi - 1 of a row, a few of them (an array) per lane at a time, all 32 lanes together; an
-// entry that a lane does not have is -inf.  The 16-byte vectors of a range are cut into steps of 256 entries; this warp
-// takes the steps part, part + parts, ... and, as the last of them, the ragged rest.  Vectors come through a ring in
-// shared memory that each lane fills and reads for itself, which keeps them in flight without registers.
+// entry that a lane does not have is -inf.  f lets the warp vote on all of them.  The 16-byte vectors of a range are cut into steps of 256 entries; the ragged
+// rest comes last.  Vectors come through a ring in shared memory that each lane fills and reads for itself, which keeps
+// them in flight without registers.
 template <typename T, typename F>
-__device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, int hi, int part, int parts, F &&f) {
-  constexpr int VEC = 16 / sizeof(T), PER = 8 / VEC, AHEAD = SL_STAGES / PER - 1; // entries per vector, vectors per step, steps in flight
+__device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, int hi, F &&f) {
+  constexpr int VEC = 16 / sizeof(T), PER = 8 / VEC, AHEAD = SL_STAGES / PER; // entries per vector, vectors per step, steps in flight
   const int lane = threadIdx.x & 31;
   if (lo >= hi) return;
   const int skip = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / static_cast<int>(sizeof(T));
@@ -143,10 +148,10 @@ __device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, in
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) fetch(part + i * parts, i);
+  for (int i = 0; i < AHEAD; ++i) fetch(i, i);
   int stage = 0;
 #pragma unroll 1
-  for (int c = part; c < steps; c += parts) {
+  for (int c = 0; c < steps; ++c) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(AHEAD - 1) : "memory");
     float v[8];
 #pragma unroll
@@ -157,12 +162,10 @@ __device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, in
       for (int i = 0; i < VEC; ++i) v[u * VEC + i] = toF32(e[i]);
     }
     f(v);
-    // the stage read in the step before this one is free: its values have been used
-    fetch(c + AHEAD * parts, stage == 0 ? AHEAD : stage - 1);
-    stage = stage == AHEAD ? 0 : stage + 1;
+    fetch(c + AHEAD, stage); // f has voted on every entry: they have arrived, the stage is free
+    stage = stage + 1 < AHEAD ? stage + 1 : 0;
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-  if (part != steps % parts) return;
   // the entries in front of the first vector and behind the last step: fewer than 8 and 256
 #pragma unroll 1
   for (int i0 = lo < a ? lo - 128 : a + steps * 256; i0 < hi; i0 = i0 < lo ? a + steps * 256 : i0 + 128) {
@@ -198,19 +201,20 @@ __device__ __forceinline__ float slMax3(float a, float b, float c) { // a NaN co
   return d;
 }
 
-// One pass over the row.  Entries in [lo, hi) go to the threads' columns; returns how many this thread found (also those
-// that did not fit).  s->pass gets the entries and (WEIGHTS) the weight at and above lo and hi (FIRST: instead of the
-// latter the weight of everything, hi being +inf) and (FIRST) the largest logit.  Comparisons run at half the rate of
-// products and sums, so a step first asks only whether any of a lane's entries can lie in the interval; few do.
-template <bool FIRST, bool WEIGHTS, typename T>
-__device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s, const Weigher &weigh, float lo, float hi) {
+// One pass over the row, a run of it per warp.  Entries in [lo, hi) go to the threads' columns; returns how many this
+// thread found (also those that did not fit).  s->pass gets the entries and (WEIGHTS) the weight at and above lo and hi
+// and (FIRST) the weight of everything and the largest logit; s->runAbove and s->runTop say the like of each run.  OPEN:
+// hi is +inf; otherwise FIRST also weighs what lies at and above `high`.  Comparisons run at half the rate of products and sums, so a step first asks only whether any of a lane's
+// entries can lie in the interval; few do.
+template <bool FIRST, bool OPEN, bool WEIGHTS, typename T>
+__device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s, const Weigher &weigh, float lo, float hi, float high) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float top = -INFINITY, fLo = 0.0f, fFrom = 0.0f, farCount = 0.0f; // farCount stays below 2^24
-  double mLo = 0.0, mFrom = 0.0;
+  float top = -INFINITY, fLo = 0.0f, fHi = 0.0f, fHigh = 0.0f, fAll = 0.0f, farCount = 0.0f; // farCount stays below 2^24
+  double mLo = 0.0, mHi = 0.0, mHigh = 0.0, mAll = 0.0;
   unsigned int mine = 0, steps = 0;
   const float middle = FIRST ? 0.0f : 0.5f * lo + 0.5f * hi, reach = FIRST ? 0.0f : fmaxf(hi - middle, middle - lo) * 1.000001f;
   float *column = &s->list[0][threadIdx.x];
-  slForRange(x, s, 0, n, warp, SL_WARPS, [&](auto &v) {
+  slForRange(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
     constexpr int N = sizeof(v) / sizeof(float);
     bool near;
     if (FIRST) {
@@ -225,18 +229,15 @@ __device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s,
       for (int i = 0; i < N; ++i) m = fminf(m, fabsf(v[i] - middle));
       near = !(m > reach);
     }
-    if (WEIGHTS) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float w = weigh(v[i]);
-        if (FIRST ? v[i] > -INFINITY : v[i] >= hi) fFrom += w;
+    for (int i = 0; i < N; ++i) {
+      const float w = WEIGHTS ? weigh(v[i]) : 0.0f;
+      if (WEIGHTS && FIRST && v[i] > -INFINITY) fAll += w;
+      if (!OPEN && v[i] >= hi) {
+        farCount += 1.0f;
+        if (WEIGHTS) fHi += w;
       }
-    }
-    if (!FIRST) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (v[i] >= hi) farCount += 1.0f;
-      }
+      if (FIRST && !OPEN && WEIGHTS && v[i] >= high) fHigh += w;
     }
     if (__any_sync(0xffffffffu, near)) {
 #pragma unroll
@@ -250,17 +251,18 @@ __device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s,
     }
     if (WEIGHTS && (++steps & 3) == 0) { // a few f32 sums at a time
       mLo += fLo;
-      mFrom += fFrom;
-      fLo = fFrom = 0.0f;
+      mHi += fHi;
+      mHigh += fHigh;
+      mAll += fAll;
+      fLo = fHi = fHigh = fAll = 0.0f;
     }
   });
   unsigned int cHi = static_cast<unsigned int>(farCount);
-  mLo += fLo;
-  mFrom += fFrom;
-  if (!FIRST) mLo += mFrom; // at and above lo
   if (WEIGHTS) {
-    mLo = slWarpSum(mLo);
-    mFrom = slWarpSum(mFrom);
+    mHi = OPEN ? 0.0 : slWarpSum(mHi + fHi);
+    mLo = slWarpSum(mLo + fLo) + mHi; // at and above lo
+    if (FIRST) mAll = slWarpSum(mAll + fAll);
+    if (FIRST && !OPEN) mHigh = slWarpSum(mHigh + fHigh);
   }
   top = slWarpMax(top);
   cHi = slWarpSum(cHi);
@@ -268,31 +270,39 @@ __device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s,
   const bool full = __any_sync(0xffffffffu, mine > SL_KEEP);
   if (lane == 0) {
     s->dRed[0][warp] = mLo;
-    s->dRed[1][warp] = mFrom;
+    s->dRed[1][warp] = s->runAbove[warp] = mHi;
+    s->dRed[2][warp] = mAll;
+    s->dRed[3][warp] = mHigh;
     s->cRed[0][warp] = cHi;
     s->cRed[1][warp] = found;
-    s->fRed[0][warp] = top;
+    s->runTop[warp] = top;
     s->iRed[warp] = full;
   }
   __syncthreads();
   if (warp == 0) {
     const int l = lane % SL_WARPS;
     mLo = s->dRed[0][l];
-    mFrom = s->dRed[1][l];
+    mHi = s->dRed[1][l];
+    mAll = s->dRed[2][l];
+    mHigh = s->dRed[3][l];
     cHi = s->cRed[0][l];
     unsigned int listed = s->cRed[1][l];
-    top = slWarpMax(s->fRed[0][l]);
+    top = slWarpMax(s->runTop[l]);
     const bool anyFull = __any_sync(0xffffffffu, s->iRed[l] != 0);
 #pragma unroll
     for (int o = SL_WARPS / 2; o > 0; o >>= 1) {
       mLo += __shfl_xor_sync(0xffffffffu, mLo, o);
-      mFrom += __shfl_xor_sync(0xffffffffu, mFrom, o);
+      mHi += __shfl_xor_sync(0xffffffffu, mHi, o);
+      mAll += __shfl_xor_sync(0xffffffffu, mAll, o);
+      mHigh += __shfl_xor_sync(0xffffffffu, mHigh, o);
       cHi += __shfl_xor_sync(0xffffffffu, cHi, o);
       listed += __shfl_xor_sync(0xffffffffu, listed, o);
     }
     if (lane == 0) {
       s->pass.mLo = mLo;
-      s->pass.mFrom = mFrom;
+      s->pass.mHi = mHi;
+      s->pass.mAll = mAll;
+      s->pass.mHigh = mHigh;
       s->pass.cHi = cHi;
       s->pass.cLo = cHi + listed;
       s->pass.fits = !anyFull;
@@ -334,7 +344,7 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
     // A range that overflows is shrunk first; one so narrow that the step overflows still separates its ends.
     const float shrink = most - least < INFINITY ? 1.0f : 0.25f, base = least * shrink, step = (SL_BINS - 1) / (most * shrink - base);
     auto binOf = [&](float v) { return max(0, min(static_cast<int>((v * shrink - base) * step), SL_BINS - 1)); };
-#pragma unroll 1
+#pragma unroll 4
     for (unsigned int i = 0; i < count; ++i) {
       const float v = column[i * SL_THREADS];
       if (v >= least && v <= most) {
@@ -369,7 +379,7 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
     rest = want - s->picked;
     // the bin's own entries; entries of one value share a bin
     float a = INFINITY, b = -INFINITY;
-#pragma unroll 1
+#pragma unroll 4
     for (unsigned int i = 0; i < count; ++i) {
       const float v = column[i * SL_THREADS];
       if (v >= least && v <= most && (bin < 0 || binOf(v) == bin)) {
@@ -409,7 +419,7 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
       most = b;
       if (!(a < b) || bin < 0) { // one value (or, without any weight, the largest one)
         unsigned int equal = 0, allEqual;
-#pragma unroll 1
+#pragma unroll 4
         for (unsigned int i = 0; i < count; ++i) equal += column[i * SL_THREADS] == b;
         slScan<unsigned int>(equal, s->cRed[0], allEqual);
         if (threadIdx.x == 0) {
@@ -427,7 +437,7 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
   unsigned long long keep = per ? (s->rest + per - 1) / per : equal, above = 0, through;
   keep = keep < 1 ? 1 : (keep > equal ? equal : keep); // a rounded limit may ask for more than there are
   if (weights) {
-#pragma unroll 1
+#pragma unroll 4
     for (unsigned int i = 0; i < count; ++i) {
       const float v = column[i * SL_THREADS];
       above += v > border ? units(v) : 0ull;
@@ -440,10 +450,11 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
 }
 
 // The next interval for a border inside [below, above): where, by the sample, `want` of the bracket's `have` entries
-// (byMass: of its weight) lie above; have <= 0: not known, the sample's estimate is taken.  Leaves s->lo and s->hi;
-// lo >= hi: the sample has nothing in the bracket.  Nothing here decides a result, only how soon it is found: f32
-// throughout.
-__device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, float above, float least, float top, bool byMass, float want, float have, int n, int samples) {
+// (byMass: of its weight) lie above; have <= 0: not known, the sample's estimate is taken.  `open`: the interval reaches up
+// to the bracket's end and down to some SL_FIRST entries.  Leaves s->lo, s->hi and
+// (s->high) where an open one would begin; lo >= hi: the sample has nothing in the bracket.  Nothing here decides a result, only how soon it is found: f32 throughout.
+__device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, float above, float least, float top, bool byMass, bool open, float want, float have, int n,
+                                         int samples) {
 #pragma unroll 1
   for (int i = threadIdx.x; i < SL_BINS; i += SL_THREADS) s->count[i] = 0;
   __syncthreads();
@@ -454,7 +465,7 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     return;
   }
   const float step = (SL_BINS - 1) / (b - a), width = (b - a) / (SL_BINS - 1);
-#pragma unroll 1
+#pragma unroll 4
   for (int i = threadIdx.x; i < samples; i += SL_THREADS) {
     const float v = s->sample[i];
     if (v >= below && v < above) atomicAdd(&s->count[min(static_cast<int>((v - a) * step + 0.5f), SL_BINS - 1)], 1u);
@@ -469,7 +480,8 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     w1 = exp2f((b1 - (SL_BINS - 1)) * width * c);
   }
   float cAll, mAll, qAll;
-  float m0 = slScan<float>(c0 + c1, s->fRed[0], cAll) + c0, m1 = m0 + c1, q0 = m0, q1 = m1;
+  const float n0 = slScan<float>(c0 + c1, s->fRed[0], cAll) + c0, n1 = n0 + c1; // entries down to either bin
+  float m0 = n0, m1 = n1, q0 = n0, q1 = n1;
   mAll = qAll = cAll;
   if (byMass) {
     m0 = slScan<float>(c0 * w0 + c1 * w1, s->fRed[1], mAll) + c0 * w0;
@@ -478,11 +490,21 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     q1 = q0 + c1 * w1 * w1;
   }
   const float perSample = static_cast<float>(n) / samples;
-  if (cAll * perSample <= 0.75f * SL_LIST) { // the whole bracket will fit
+  if (cAll * perSample <= 0.6f * SL_LIST) { // the whole bracket will fit
     if (threadIdx.x == 0) {
       s->lo = below;
       s->hi = above;
     }
+    __syncthreads();
+    return;
+  }
+  const float enough = SL_FIRST / perSample;
+  const bool at0 = n0 >= enough && n0 - c0 < enough, at1 = n1 >= enough && n0 < enough;
+  if (at0 || at1) { // the first bin down to which there are enough: one thread's
+    s->high = s->lo = fmaxf(below, a + ((at0 ? b0 : b1) - 0.5f) * width);
+    s->hi = above;
+  }
+  if (open) {
     __syncthreads();
     return;
   }
@@ -511,15 +533,18 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
     }
     __syncthreads();
     const int pLo = s->pickBin[0], pHi = s->pickBin[1];
-    unsigned int inside = 0, sum;
-    if (b0 >= pLo && b0 < pHi) inside += s->count[b0];
-    if (b1 >= pLo && b1 < pHi) inside += s->count[b1];
-    slScan<unsigned int>(inside, s->cRed[0], sum);
+    // how many the interval would hold, and how many with everything above it (two 16-bit counts)
+    unsigned int inside = 0, both;
+    if (b0 >= pLo) inside += s->count[b0] * (b0 < pHi ? 0x10001u : 0x10000u);
+    if (b1 >= pLo) inside += s->count[b1] * (b1 < pHi ? 0x10001u : 0x10000u);
+    slScan<unsigned int>(inside, s->cRed[0], both);
+    const unsigned int sum = both & 0xffffu;
+    const bool up = (both >> 16) * perSample <= 0.6f * SL_LIST; // the sample says little about a few heavy entries
     if (sum * perSample <= SL_LIST || pHi - pLo <= 1 || round == 3) {
       // bin edges lie half a bin below the bins' middles; open ends reach to the bracket's
       if (threadIdx.x == 0) {
         s->lo = pLo < 0 ? below : fmaxf(below, a + (pLo - 0.5f) * width);
-        s->hi = pHi >= SL_BINS ? above : fminf(above, a + (pHi - 0.5f) * width);
+        s->hi = up || pHi >= SL_BINS ? above : fminf(above, a + (pHi - 0.5f) * width);
       }
       __syncthreads();
       return;
@@ -528,84 +553,125 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
   }
 }
 
-// The draw among the entries above `border` and the first `ties` equal to it, with a weight of at least `low`: weigh
-// 16 runs, go into the one that holds u times the total, until 32 entries are left.  False: the total is out of range.
+// The draw among the entries above `border` and the first `ties` equal to it, with a weight of at least `low`.  The row is
+// weighed by the 16 runs of slPass, the run that holds u times the total by a part per thread, and so on until 32 entries
+// are left.  The last pass may have left what is needed of the runs: KNOWN_LIST, this thread's `count` entries (all that
+// stay below hi) and s->runAbove (times `scale`); KNOWN_TOP, s->runTop (the first of the largest logits is drawn).
+// False: the total is out of range.
 template <typename T>
-__device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const Weigher &weigh, float border, unsigned int ties, float low, double u, int32_t *out,
-                                    float *prob) {
+__device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const Weigher &weigh, float border, unsigned int ties, float low, double u, int known,
+                                       unsigned int count, double scale, int32_t *out, float *prob) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float wBorder = border < INFINITY ? (border > -INFINITY ? weigh(border) : 0.0f) : 1.0f;
   const double wEqual = wBorder >= low ? static_cast<double>(wBorder) : 0.0;
-  int from = 0, to = n;
-  bool whole = true;
-  for (;;) {
-    const int part = whole ? 0 : (to - from + SL_WARPS - 1) / SL_WARPS;
-    const int lo = whole ? slRun(n, warp) : min(to, from + warp * part), hi = whole ? slRun(n, warp + 1) : min(to, lo + part);
-    double sum = 0.0;
-    float f = 0.0f;
-    unsigned int equal = 0;
-    unsigned int steps = 0;
-    slForRange(x, s, lo, hi, 0, 1, [&](auto &v) {
+  double sum = 0.0;
+  float f = 0.0f;
+  unsigned int equal = 0, steps = 0;
+  auto weighUp = [&](float v) {
+    const float w = weigh(v);
+    if (v > border && !(w < low)) f += w; // an overflowed weight (inf, or NaN) must show in the total
+    return v == border;
+  };
+  if (known == KNOWN_LIST) { // at most SL_KEEP of them
+#pragma unroll 1
+    for (unsigned int i = 0; i < count; ++i) equal += weighUp(s->list[i][threadIdx.x]);
+  } else if (known == KNOWN_TOP) {
+    equal = lane == 0 && s->runTop[warp] == border;
+  } else {
+    slForRange(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
       constexpr int N = sizeof(v) / sizeof(float);
+      bool any = false;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float w = weigh(v[i]);
-        if (v[i] > border && !(w < low)) f += w; // an overflowed weight (inf, or NaN) must show in the total
-        if (v[i] == border) ++equal;
+      for (int i = 0; i < N; ++i) any |= weighUp(v[i]);
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) equal += v[i] == border;
       }
       if ((++steps & 3) == 0) {
         sum += f;
         f = 0.0f;
       }
     });
-    sum += f;
-    sum = slWarpSum(sum);
-    equal = slWarpSum(equal);
-    if (lane == 0) {
-      s->dRed[0][warp] = sum;
-      s->cRed[0][warp] = equal;
+  }
+  sum = slWarpSum(sum + f);
+  equal = slWarpSum(equal);
+  if (lane == 0) {
+    s->dRed[0][warp] = known == KNOWN_LIST ? sum + s->runAbove[warp] * scale : sum;
+    s->cRed[0][warp] = equal;
+  }
+  __syncthreads();
+  if (warp == 0) { // lane w: run w
+    const bool mine = lane < SL_WARPS;
+    const unsigned int eq = mine ? s->cRed[0][lane] : 0u, seen = slWarpScan(eq) - eq;
+    const unsigned int stay = seen < ties ? min(eq, ties - seen) : 0u;
+    const double m = mine ? s->dRed[0][lane] + wEqual * stay : 0.0;
+    const double run = slWarpScan(m);
+    const double total = __shfl_sync(0xffffffffu, run, 31), target = u * total;
+    const unsigned int hit = __ballot_sync(0xffffffffu, m > 0.0 && run > target), any = __ballot_sync(0xffffffffu, m > 0.0);
+    // none: u = 1, or the last bit of a sum taken in another order: the last run that weighs anything
+    const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : SL_WARPS - 1);
+    if (lane == at) {
+      s->target = target - (run - m);
+      s->equalBefore = seen;
+      s->from = slRun(n, lane);
+      s->to = slRun(n, lane + 1);
+      s->total = total;
+      s->ok = total > 0.0 && total < 1e300;
     }
-    __syncthreads();
-    if (warp == 0) { // lane w: run w
-      const bool mine = lane < SL_WARPS;
-      const unsigned long long eq = mine ? s->cRed[0][lane] : 0ull;
-      unsigned long long seen = slWarpScan(eq) - eq + (whole ? 0ull : s->equalBefore);
-      const unsigned long long stay = seen < ties ? (eq < ties - seen ? eq : ties - seen) : 0ull;
-      const double m = mine ? s->dRed[0][lane] + wEqual * static_cast<double>(stay) : 0.0;
-      const double run = slWarpScan(m);
-      const double total = __shfl_sync(0xffffffffu, run, 31);
-      const double target = whole ? u * total : s->target;
-      const unsigned int hit = __ballot_sync(0xffffffffu, m > 0.0 && run > target), any = __ballot_sync(0xffffffffu, m > 0.0);
-      // none: u = 1, or the last bit of a sum taken in another order: the last run that weighs anything
-      const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : SL_WARPS - 1);
-      if (lane == at) {
-        s->target = target - (run - m);
-        s->equalBefore = seen;
-        const int nf = whole ? slRun(n, lane) : min(to, from + lane * part);
-        s->from = nf;
-        s->to = whole ? slRun(n, lane + 1) : min(to, nf + part);
-        if (whole) {
-          s->total = total;
-          s->ok = total > 0.0 && total < 1e300;
-        }
+  }
+  __syncthreads();
+  if (!s->ok) return false;
+  int from = s->from, to = s->to;
+  while (to - from > 32) {
+    const int part = (to - from + SL_THREADS - 1) / SL_THREADS, lo = min(to, from + static_cast<int>(threadIdx.x) * part), hi = min(to, lo + part);
+    const double target = s->target;
+    const unsigned int equalBefore = s->equalBefore;
+    if (threadIdx.x == 0) {
+      s->pickBin[0] = SL_THREADS;
+      s->pickBin[1] = 0;
+    }
+    sum = 0.0;
+    equal = 0;
+#pragma unroll 1
+    for (int i0 = lo; i0 < hi; i0 += 16) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = i0 + i < hi ? fmaxf(toF32(x[i0 + i]), -INFINITY) : -INFINITY;
+      f = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (i0 + i < hi) equal += weighUp(v[i]);
       }
+      sum += f;
+    }
+    unsigned int allEqual;
+    double all;
+    const unsigned int seen = equalBefore + slScan<unsigned int>(equal, s->cRed[0], allEqual), stay = seen < ties ? min(equal, ties - seen) : 0u;
+    const double m = sum + wEqual * stay, before = slScan<double>(m, s->dRed[0], all);
+    if (m > 0.0) {
+      if (before + m > target) atomicMin(&s->pickBin[0], static_cast<int>(threadIdx.x));
+      atomicMax(&s->pickBin[1], static_cast<int>(threadIdx.x));
     }
     __syncthreads();
-    if (!s->ok) return false;
+    if (static_cast<int>(threadIdx.x) == (s->pickBin[0] < SL_THREADS ? s->pickBin[0] : s->pickBin[1])) {
+      s->target = target - before;
+      s->equalBefore = seen;
+      s->from = lo;
+      s->to = hi;
+    }
+    __syncthreads();
     from = s->from;
     to = s->to;
-    whole = false;
-    if (to - from <= 32) break;
     __syncthreads();
   }
   if (warp == 0) {
     const int i = from + lane;
     const float v = i < to ? fmaxf(toF32(x[i]), -INFINITY) : -INFINITY;
     const float w = weigh(v);
-    const bool equal = i < to && v == border;
-    const unsigned int eq = __ballot_sync(0xffffffffu, equal);
-    const unsigned long long rank = s->equalBefore + __popc(eq & ((1u << lane) - 1u));
-    const double mine = v > border && !(w < low) ? static_cast<double>(w) : (equal && rank < ties ? wEqual : 0.0);
+    const bool same = i < to && v == border;
+    const unsigned int eq = __ballot_sync(0xffffffffu, same);
+    const unsigned int rank = s->equalBefore + __popc(eq & ((1u << lane) - 1u));
+    const double mine = v > border && !(w < low) ? static_cast<double>(w) : (same && rank < ties ? wEqual : 0.0);
     const double run = slWarpScan(mine);
     const unsigned int hit = __ballot_sync(0xffffffffu, mine > 0.0 && run > s->target), any = __ballot_sync(0xffffffffu, mine > 0.0);
     const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : 0);
@@ -641,19 +707,32 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
   const float low = !greedy && minP && minP[row] > 0.0f && minP[row] <= 1.0f ? minP[row] : 0.0f;
   const double u = fmin(fmax(static_cast<double>(uniform[row]), 0.0), 1.0); // NaN: 0
 
-  // ---- a sample: evenly spaced entries, or all of a short row
+  // ---- a sample: evenly spaced, or all of a short row
   const int samples = min(n, SL_SAMPLE);
-  const float stride = static_cast<float>(n) / samples;
   float sTop = -INFINITY, sLeast = INFINITY; // of the finite ones
+  auto take = [&](int at, float v) {
+    v = fmaxf(v, -INFINITY);
+    s->sample[at] = v;
+    sTop = fmaxf(sTop, v);
+    if (v > -INFINITY) sLeast = fminf(sLeast, v);
+  };
+  if (n >= 4 * SL_SAMPLE) { // 16-byte vectors: a single entry would cost the memory a whole sector
+    constexpr int VEC = 16 / sizeof(T), SPOTS = SL_SAMPLE / VEC;
+    const int a = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T));
+    const int apart = (n - a) / VEC / SPOTS;
+    uint4 raw[SPOTS / SL_THREADS];
 #pragma unroll
-  for (int i = 0; i < SL_SAMPLE / SL_THREADS; ++i) {
-    const int e = tid + i * SL_THREADS;
-    if (e < samples) {
-      const float v = fmaxf(toF32(x[min(n - 1, static_cast<int>(e * stride))]), -INFINITY);
-      s->sample[e] = v;
-      sTop = fmaxf(sTop, v);
-      if (v > -INFINITY) sLeast = fminf(sLeast, v);
+    for (int i = 0; i < SPOTS / SL_THREADS; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(x + a) + (tid + i * SL_THREADS) * apart);
+#pragma unroll
+    for (int i = 0; i < SPOTS / SL_THREADS; ++i) {
+      const T *e = reinterpret_cast<const T *>(&raw[i]);
+#pragma unroll
+      for (int k2 = 0; k2 < VEC; ++k2) take((i * VEC + k2) * SL_THREADS + tid, toF32(e[k2]));
     }
+  } else {
+    const float stride = static_cast<float>(n) / samples;
+#pragma unroll 1
+    for (int e = tid; e < samples; e += SL_THREADS) take(e, toF32(x[min(n - 1, static_cast<int>(e * stride))]));
   }
   __syncthreads();
   slSpan(s, sLeast, sTop);
@@ -667,23 +746,28 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
   bool exactTop = false, search = cut || greedy || low > 0.0f || !(sTop > -INFINITY && sTop < INFINITY);
   weigh.refer(sTop, greedy ? 1.0f : heat);
   for (;;) {
+    int known = KNOWN_NOTHING;
+    unsigned int listed = 0; // entries this thread collected in the last pass
+    double scale = 1.0;      // of that pass's weights to the present reference
     if (search) {
       // The list holds the entries in [lo, hi); the border of the cut at work lies in [below, above).
-      bool first = true, again = false, byMass = false, infinite = false;
+      bool first = true, again = false, byMass = false, infinite = false, up = false;
       bool ask = cut && n > SL_SHORT && sTop > -INFINITY && sTop < INFINITY; // choose an interval first
       float below = fmaxf(fmaxf(sTop - SL_FLOOR / weigh.c, -FLT_MAX), sLeast), above = INFINITY, floor = below, top = sTop;
-      float lo = cut ? -FLT_MAX : INFINITY, hi = INFINITY, want = SL_FIRST, have = 0.0f, firstLo = INFINITY, borderK = -INFINITY;
+      float lo = cut ? -FLT_MAX : INFINITY, hi = INFINITY, want = static_cast<float>(k), have = 0.0f, firstLo = INFINITY, firstHi = INFINITY, high = INFINITY, borderK = -INFINITY;
       unsigned int tiesK = 0xffffffffu;
-      double firstMass = 0.0;
+      double firstMass = 0.0, firstHiMass = 0.0, highMass = 0.0;
       double total = 0.0, atBelow = 0.0, atAbove = 0.0, limit = 0.0, mLo = 0.0, mHi = 0.0;
       int which = cutK ? 0 : 1, round = 0;
       for (bool done = false; !done;) {
         if (ask) {
-          slChoose(s, weigh.c, below, above, sLeast, top, byMass, want, have, n, samples);
+          // The first interval is open unless top-k is too deep for that.
+          slChoose(s, weigh.c, below, above, sLeast, top, byMass, first ? !cutK || want <= 0.6f * SL_FIRST : up, want, have, n, samples);
           float nLo = s->lo, nHi = s->hi;
-          if (first) { // open above, so that it finds the largest logit
+          if (first) {
             nLo = fminf(nLo, sTop);
-            nHi = INFINITY;
+            if (!(nLo < nHi)) nHi = INFINITY;
+            if (nHi < INFINITY) high = fmaxf(s->high, nHi);
           } else if (!(nLo < nHi) || (nLo == lo && nHi == hi) || round >= 10) {
             // no help from the sample, or just what did not fit: halve the bracket in the order of the floats
             auto order = [](float v) {
@@ -701,9 +785,10 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           lo = first ? nLo : fmaxf(nLo, below);
           hi = fminf(nHi, above);
         }
-        unsigned int mine;
-        if (first && !infinite) mine = cutP ? slPass<true, true>(x, n, s, weigh, lo, hi) : slPass<true, false>(x, n, s, weigh, lo, hi);
-        else mine = cutP ? slPass<false, true>(x, n, s, weigh, lo, hi) : slPass<false, false>(x, n, s, weigh, lo, hi);
+        if (!first || infinite) listed = slPass<false, false, true>(x, n, s, weigh, lo, hi, INFINITY);
+        else if (hi < INFINITY) listed = slPass<true, false, true>(x, n, s, weigh, lo, hi, high);
+        else if (cutP) listed = slPass<true, true, true>(x, n, s, weigh, lo, hi, INFINITY);
+        else listed = slPass<true, true, false>(x, n, s, weigh, lo, hi, INFINITY);
         const PassResult cur = s->pass;
         if (infinite) { // only the infinite ones weigh anything: both cuts count them
           border = INFINITY;
@@ -726,42 +811,46 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           if (greedy) {
             border = cur.top;
             ties = 1;
+            known = KNOWN_TOP;
             break;
           }
           if (cur.top == INFINITY) {
             infinite = true;
             ask = false;
-            lo = INFINITY;
+            lo = hi = INFINITY;
             continue;
           }
           if (!cut) break;
           // From here on weights are relative to the true largest logit; the first pass's are rescaled, or taken again
           // when its reference was so far off that they may have overflowed (or there was none).
-          double rescale = 1.0;
-          if (!again && cutP) {
+          if (!again && (cutP || hi < INFINITY)) {
             if (!(rise < 60.0)) {
               again = true;
               ask = false;
               continue;
             }
-            rescale = static_cast<double>(exp2f(static_cast<float>(-rise)));
+            scale = static_cast<double>(exp2f(static_cast<float>(-rise)));
           }
           first = false;
           top = cur.top;
           floor = fmaxf(top - SL_FLOOR / weigh.c, -FLT_MAX);
-          total = cur.mFrom * rescale;
-          mHi = 0.0;
-          mLo = cur.mLo * rescale;
+          total = cur.mAll * scale;
+          mHi = cur.mHi * scale;
+          mLo = cur.mLo * scale;
           byMass = which == 1;
           limit = byMass ? static_cast<double>(p) * total : static_cast<double>(k);
           firstLo = lo;
           firstMass = mLo;
+          firstHi = hi;
+          firstHiMass = mHi;
+          highMass = hi < INFINITY ? cur.mHigh * scale : 0.0;
           below = floor;
           above = nextafterf(top, INFINITY);
           atBelow = byMass ? total : 0.0; // entries: not known yet
         } else {
-          mHi = cur.mFrom;
+          mHi = cur.mHi;
           mLo = cur.mLo;
+          scale = 1.0;
         }
         __syncthreads(); // everyone has read the pass's result
         ask = true;
@@ -770,12 +859,15 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
         while (ask && !done) {
           const double hiAt = byMass ? mHi : static_cast<double>(cur.cHi), loAt = byMass ? mLo : static_cast<double>(cur.cLo);
           bool found = false;
+          known = KNOWN_NOTHING;
+          up = false;
           if (limit > hiAt && limit <= loAt) {
             if (cur.fits) {
               const double rest = byMass ? ceil((limit - hiAt) * static_cast<double>(SL_UNIT)) : limit - hiAt;
-              slSelect(s, weigh, mine, byMass, cutP, static_cast<unsigned long long>(fmax(rest, 1.0)), lo, fminf(hi, top));
+              slSelect(s, weigh, listed, byMass, cutP, static_cast<unsigned long long>(fmax(rest, 1.0)), lo, fminf(hi, top));
               border = s->border;
               ties = s->ties;
+              known = KNOWN_LIST;
               total = mHi + static_cast<double>(s->through) / static_cast<double>(SL_UNIT);
               found = true;
             } else {
@@ -805,6 +897,7 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           } else if (hi > below) { // further up
             below = hi;
             atBelow = hiAt;
+            up = byMass; // a few heavy entries, of which the sample says little
           }
           if (!found && (above <= below || round >= 100)) { // sums that differ in their last bits left nothing between: here it is
             border = below;
@@ -826,12 +919,31 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
             atBelow = total;
             atAbove = 0.0;
             round = 0;
-            if (limit > firstMass) { // what the first pass knows: the sample says little about a few heavy entries
+            up = false;
+            if (limit > firstMass) { // what the first pass knows
               above = fminf(above, firstLo);
               atAbove = firstMass;
-            } else if (firstLo > below) {
-              below = firstLo;
-              atBelow = firstMass;
+            } else if (limit > firstHiMass) {
+              if (firstHi < above) {
+                above = firstHi;
+                atAbove = firstHiMass;
+              }
+              if (firstLo > below) {
+                below = firstLo;
+                atBelow = firstMass;
+              }
+            } else {
+              if (firstHi > below) {
+                below = firstHi;
+                atBelow = firstHiMass;
+              }
+              if (limit > highMass) { // the heaviest entries, of which the sample says little, are out of the way
+                above = fminf(above, high);
+                atAbove = highMass;
+              } else if (high > below) {
+                below = high;
+                atBelow = highMass;
+              }
             }
           }
         }
@@ -841,9 +953,12 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
       if (cut && border < floor) {
         border = floor;
         ties = 0xffffffffu;
+        known = KNOWN_NOTHING;
       }
+      // What lies above the list must stay as a whole: a min-p that may reach into it asks for another look.
+      if (known == KNOWN_LIST && hi < INFINITY && !(weigh(hi) > 1.0001f * low)) known = KNOWN_NOTHING;
     }
-    if (slPick(x, n, s, weigh, border, ties, low, u, out, prob) || exactTop) return;
+    if (slPick(x, n, s, weigh, border, ties, low, u, known, listed, scale, out, prob) || exactTop) return;
     search = true; // nothing was cut, and the sample's largest logit was too small a reference
     __syncthreads();
   }
