@@ -17,8 +17,8 @@
 //    the border and the next interval is chosen inside the bracket, so the search always ends.  The first interval is
 //    open above and sized for some 2500 entries, which answers most top-k and top-p settings at once and finds the
 //    largest logit on the way.
-//  * The draw is a search too: of the warps' runs the one that holds u times the total, of it the thread's part that
-//    does, until 32 entries are left.  After a cut the last pass knows the runs' weights already.
+//  * The draw is a search too: of the warps' runs the one that holds u times the total is split among the warps
+//    again, until there is a thread for each entry.  After a cut the last pass knows the runs' weights already.
 // What bounds it: instruction issue, at some 10 instructions per entry and pass.
 #include "common.cuh"
 
@@ -554,8 +554,8 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
 }
 
 // The draw among the entries above `border` and the first `ties` equal to it, with a weight of at least `low`.  The row is
-// weighed by the 16 runs of slPass, the run that holds u times the total by a part per thread, and so on until 32 entries
-// are left.  The last pass may have left what is needed of the runs: KNOWN_LIST, this thread's `count` entries (all that
+// weighed by the 16 runs of slPass, the run that holds u times the total by 16 runs again, until there is a thread for
+// each entry that is left.  The last pass may have left what is needed of the runs: KNOWN_LIST, this thread's `count` entries (all that
 // stay below hi) and s->runAbove (times `scale`); KNOWN_TOP, s->runTop (the first of the largest logits is drawn).
 // False: the total is out of range.
 template <typename T>
@@ -564,121 +564,108 @@ __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const W
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float wBorder = border < INFINITY ? (border > -INFINITY ? weigh(border) : 0.0f) : 1.0f;
   const double wEqual = wBorder >= low ? static_cast<double>(wBorder) : 0.0;
-  double sum = 0.0;
   float f = 0.0f;
-  unsigned int equal = 0, steps = 0;
   auto weighUp = [&](float v) {
     const float w = weigh(v);
     if (v > border && !(w < low)) f += w; // an overflowed weight (inf, or NaN) must show in the total
     return v == border;
   };
-  if (known == KNOWN_LIST) { // at most SL_KEEP of them
+  int from = 0, to = n;
+  for (bool whole = true; whole || to - from > SL_THREADS; whole = false) {
+    const int part = (to - from + SL_WARPS - 1) / SL_WARPS;
+    double sum = 0.0;
+    unsigned int equal = 0, steps = 0;
+    f = 0.0f;
+    if (!whole) {
+      const int lo = min(to, from + warp * part), hi = min(to, lo + part);
 #pragma unroll 1
-    for (unsigned int i = 0; i < count; ++i) equal += weighUp(s->list[i][threadIdx.x]);
-  } else if (known == KNOWN_TOP) {
-    equal = lane == 0 && s->runTop[warp] == border;
-  } else {
-    slForRange(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
-      constexpr int N = sizeof(v) / sizeof(float);
-      bool any = false;
+      for (int i0 = lo + lane; i0 < hi; i0 += 32 * 16) {
+        float v[16];
 #pragma unroll
-      for (int i = 0; i < N; ++i) any |= weighUp(v[i]);
-      if (__any_sync(0xffffffffu, any)) {
+        for (int i = 0; i < 16; ++i) v[i] = i0 + 32 * i < hi ? fmaxf(toF32(x[i0 + 32 * i]), -INFINITY) : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < N; ++i) equal += v[i] == border;
-      }
-      if ((++steps & 3) == 0) {
+        for (int i = 0; i < 16; ++i) equal += weighUp(v[i]) && i0 + 32 * i < hi;
         sum += f;
         f = 0.0f;
       }
-    });
-  }
-  sum = slWarpSum(sum + f);
-  equal = slWarpSum(equal);
-  if (lane == 0) {
-    s->dRed[0][warp] = known == KNOWN_LIST ? sum + s->runAbove[warp] * scale : sum;
-    s->cRed[0][warp] = equal;
-  }
-  __syncthreads();
-  if (warp == 0) { // lane w: run w
-    const bool mine = lane < SL_WARPS;
-    const unsigned int eq = mine ? s->cRed[0][lane] : 0u, seen = slWarpScan(eq) - eq;
-    const unsigned int stay = seen < ties ? min(eq, ties - seen) : 0u;
-    const double m = mine ? s->dRed[0][lane] + wEqual * stay : 0.0;
-    const double run = slWarpScan(m);
-    const double total = __shfl_sync(0xffffffffu, run, 31), target = u * total;
-    const unsigned int hit = __ballot_sync(0xffffffffu, m > 0.0 && run > target), any = __ballot_sync(0xffffffffu, m > 0.0);
-    // none: u = 1, or the last bit of a sum taken in another order: the last run that weighs anything
-    const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : SL_WARPS - 1);
-    if (lane == at) {
-      s->target = target - (run - m);
-      s->equalBefore = seen;
-      s->from = slRun(n, lane);
-      s->to = slRun(n, lane + 1);
-      s->total = total;
-      s->ok = total > 0.0 && total < 1e300;
-    }
-  }
-  __syncthreads();
-  if (!s->ok) return false;
-  int from = s->from, to = s->to;
-  while (to - from > 32) {
-    const int part = (to - from + SL_THREADS - 1) / SL_THREADS, lo = min(to, from + static_cast<int>(threadIdx.x) * part), hi = min(to, lo + part);
-    const double target = s->target;
-    const unsigned int equalBefore = s->equalBefore;
-    if (threadIdx.x == 0) {
-      s->pickBin[0] = SL_THREADS;
-      s->pickBin[1] = 0;
-    }
-    sum = 0.0;
-    equal = 0;
-#pragma unroll 1
-    for (int i0 = lo; i0 < hi; i0 += 16) {
-      float v[16];
+    } else if (known == KNOWN_LIST) { // at most SL_KEEP of them
+#pragma unroll 4
+      for (unsigned int i = 0; i < count; ++i) equal += weighUp(s->list[i][threadIdx.x]);
+    } else if (known == KNOWN_TOP) {
+      equal = lane == 0 && s->runTop[warp] == border;
+    } else {
+      slForRange(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
+        constexpr int N = sizeof(v) / sizeof(float);
+        bool any = false;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = i0 + i < hi ? fmaxf(toF32(x[i0 + i]), -INFINITY) : -INFINITY;
-      f = 0.0f;
+        for (int i = 0; i < N; ++i) any |= weighUp(v[i]);
+        if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (i0 + i < hi) equal += weighUp(v[i]);
+          for (int i = 0; i < N; ++i) equal += v[i] == border;
+        }
+        if ((++steps & 3) == 0) {
+          sum += f;
+          f = 0.0f;
+        }
+      });
+    }
+    sum = slWarpSum(sum + f);
+    equal = slWarpSum(equal);
+    if (lane == 0) {
+      s->dRed[0][warp] = whole && known == KNOWN_LIST ? sum + s->runAbove[warp] * scale : sum;
+      s->cRed[0][warp] = equal;
+    }
+    __syncthreads();
+    if (warp == 0) { // lane w: run w
+      const bool mine = lane < SL_WARPS;
+      const unsigned int eq = mine ? s->cRed[0][lane] : 0u, seen = slWarpScan(eq) - eq + (whole ? 0u : s->equalBefore);
+      const unsigned int stay = seen < ties ? min(eq, ties - seen) : 0u;
+      const double m = mine ? s->dRed[0][lane] + wEqual * stay : 0.0;
+      const double run = slWarpScan(m);
+      const double total = __shfl_sync(0xffffffffu, run, 31), target = whole ? u * total : s->target;
+      const unsigned int hit = __ballot_sync(0xffffffffu, m > 0.0 && run > target), any = __ballot_sync(0xffffffffu, m > 0.0);
+      // none: u = 1, or the last bit of a sum taken in another order: the last run that weighs anything
+      const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : SL_WARPS - 1);
+      if (lane == at) {
+        s->target = target - (run - m);
+        s->equalBefore = seen;
+        const int lo = whole ? slRun(n, lane) : min(to, from + lane * part);
+        s->from = lo;
+        s->to = whole ? slRun(n, lane + 1) : min(to, lo + part);
+        if (whole) {
+          s->total = total;
+          s->ok = total > 0.0 && total < 1e300;
+        }
       }
-      sum += f;
-    }
-    unsigned int allEqual;
-    double all;
-    const unsigned int seen = equalBefore + slScan<unsigned int>(equal, s->cRed[0], allEqual), stay = seen < ties ? min(equal, ties - seen) : 0u;
-    const double m = sum + wEqual * stay, before = slScan<double>(m, s->dRed[0], all);
-    if (m > 0.0) {
-      if (before + m > target) atomicMin(&s->pickBin[0], static_cast<int>(threadIdx.x));
-      atomicMax(&s->pickBin[1], static_cast<int>(threadIdx.x));
     }
     __syncthreads();
-    if (static_cast<int>(threadIdx.x) == (s->pickBin[0] < SL_THREADS ? s->pickBin[0] : s->pickBin[1])) {
-      s->target = target - before;
-      s->equalBefore = seen;
-      s->from = lo;
-      s->to = hi;
-    }
-    __syncthreads();
+    if (!s->ok) return false;
     from = s->from;
     to = s->to;
     __syncthreads();
   }
-  if (warp == 0) {
-    const int i = from + lane;
-    const float v = i < to ? fmaxf(toF32(x[i]), -INFINITY) : -INFINITY;
-    const float w = weigh(v);
-    const bool same = i < to && v == border;
-    const unsigned int eq = __ballot_sync(0xffffffffu, same);
-    const unsigned int rank = s->equalBefore + __popc(eq & ((1u << lane) - 1u));
-    const double mine = v > border && !(w < low) ? static_cast<double>(w) : (same && rank < ties ? wEqual : 0.0);
-    const double run = slWarpScan(mine);
-    const unsigned int hit = __ballot_sync(0xffffffffu, mine > 0.0 && run > s->target), any = __ballot_sync(0xffffffffu, mine > 0.0);
-    const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : 0);
-    if (lane == at) {
-      *out = any ? i : -1;
-      if (prob) *prob = any ? static_cast<float>(mine / s->total) : 0.0f;
-    }
+  // a thread per entry
+  if (threadIdx.x == 0) {
+    s->pickBin[0] = SL_THREADS;
+    s->pickBin[1] = -1;
+  }
+  const int i = from + static_cast<int>(threadIdx.x);
+  const float v = i < to ? fmaxf(toF32(x[i]), -INFINITY) : -INFINITY;
+  f = 0.0f;
+  const bool same = weighUp(v) && i < to;
+  unsigned int allSame;
+  double all;
+  const unsigned int rank = s->equalBefore + slScan<unsigned int>(same, s->cRed[0], allSame);
+  const double mine = same ? (rank < ties ? wEqual : 0.0) : static_cast<double>(f), before = slScan<double>(mine, s->dRed[0], all);
+  if (mine > 0.0) {
+    if (before + mine > s->target) atomicMin(&s->pickBin[0], static_cast<int>(threadIdx.x));
+    atomicMax(&s->pickBin[1], static_cast<int>(threadIdx.x));
+  }
+  __syncthreads();
+  const int at = s->pickBin[0] < SL_THREADS ? s->pickBin[0] : max(s->pickBin[1], 0);
+  if (static_cast<int>(threadIdx.x) == at) {
+    *out = s->pickBin[1] >= 0 ? i : -1;
+    if (prob) *prob = s->pickBin[1] >= 0 ? static_cast<float>(mine / s->total) : 0.0f;
   }
   return true;
 }
