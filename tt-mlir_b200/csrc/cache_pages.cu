@@ -70,11 +70,13 @@ __global__ void __launch_bounds__(PG_THREADS)
   }
 }
 
-// grid: x = piece of a user's [nodes, heads, row] items, y = user, z = cache.  Item i of the path goes to position
-// lens[b] + i.
+// grid: x = piece of a user's [nodes, heads, row] items, y = user, z = group of caches.  Item i of the path goes to
+// position lens[b] + i.  Where a unit comes from and goes to is the same in every cache and costs a chain of dependent
+// loads (length, path, page), so a CTA finds it once and then moves its units in one cache after the other, the next
+// cache's loads in front of this one's stores.
 template <typename U>
 __global__ void __launch_bounds__(PG_THREADS)
-    commitDraftKernel(DraftPointers ptrs, const int32_t *__restrict__ table, const int32_t *__restrict__ lens, const int32_t *__restrict__ path,
+    commitDraftKernel(DraftPointers ptrs, int caches, const int32_t *__restrict__ table, const int32_t *__restrict__ lens, const int32_t *__restrict__ path,
                       const int32_t *__restrict__ pathLens, int nodes, int heads, int64_t blocks, int blockSize, int pages, int rowUnits, int *bad) {
   pdlLaunchDependents();
   pdlWait();
@@ -83,31 +85,48 @@ __global__ void __launch_bounds__(PG_THREADS)
   const int64_t total = static_cast<int64_t>(count) * perNode;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (PG_THREADS * PG_UNROLL);
   if (first >= total) return;
-  const U *draft = static_cast<const U *>(ptrs.draft[blockIdx.z]) + static_cast<int64_t>(b) * nodes * perNode;
-  U *cache = static_cast<U *>(ptrs.cache[blockIdx.z]);
   const int64_t len = lens[b];
-  U r[PG_UNROLL];
-  int64_t dst[PG_UNROLL];
+  int64_t src[PG_UNROLL], dst[PG_UNROLL];
 #pragma unroll
   for (int i = 0; i < PG_UNROLL; ++i) {
     const int64_t at = first + i * PG_THREADS + threadIdx.x;
     dst[i] = -1;
     if (at >= total) continue;
-    const int step = static_cast<int>(at / perNode), rem = static_cast<int>(at % perNode), h = rem / rowUnits, u = rem % rowUnits;
+    const bool small = total <= 0x7fffffff; // a 64-bit division costs several times a 32-bit one
+    const int step = small ? static_cast<int>(at) / perNode : static_cast<int>(at / perNode);
+    const int rem = static_cast<int>(at - static_cast<int64_t>(step) * perNode), h = rem / rowUnits, u = rem % rowUnits;
     const int node = path[static_cast<int64_t>(b) * nodes + step];
-    const int64_t pos = len + step, page = pos / blockSize;
+    const int64_t pos = len + step;
+    const int64_t page = pos <= 0x7fffffff ? static_cast<int>(pos) / blockSize : pos / blockSize;
     int blk = -1;
     if (len >= 0 && page < pages) blk = table[static_cast<int64_t>(b) * pages + page];
     if (node < 0 || node >= nodes || blk < 0 || blk >= blocks) { // nowhere to go: left out and reported
       *bad = 1;
       continue;
     }
-    r[i] = draft[static_cast<int64_t>(node) * perNode + rem];
-    dst[i] = ((blk * static_cast<int64_t>(heads) + h) * blockSize + pos % blockSize) * rowUnits + u;
+    src[i] = (static_cast<int64_t>(b) * nodes + node) * perNode + rem;
+    dst[i] = ((blk * static_cast<int64_t>(heads) + h) * blockSize + (pos - page * blockSize)) * rowUnits + u;
   }
+  U r[PG_UNROLL], next[PG_UNROLL];
+  auto load = [&](U *to, const void *draft) {
 #pragma unroll
-  for (int i = 0; i < PG_UNROLL; ++i) {
-    if (dst[i] >= 0) cache[dst[i]] = r[i];
+    for (int i = 0; i < PG_UNROLL; ++i) {
+      if (dst[i] >= 0) to[i] = static_cast<const U *>(draft)[src[i]];
+    }
+  };
+  int c = blockIdx.z;
+  load(r, ptrs.draft[c]);
+  for (;;) {
+    const int after = c + gridDim.z;
+    if (after < caches) load(next, ptrs.draft[after]);
+    U *cache = static_cast<U *>(ptrs.cache[c]);
+#pragma unroll
+    for (int i = 0; i < PG_UNROLL; ++i) {
+      if (dst[i] >= 0) cache[dst[i]] = r[i];
+      r[i] = next[i];
+    }
+    if (after >= caches) return;
+    c = after;
   }
 }
 
@@ -203,8 +222,11 @@ int ttb_paged_commit_draft(void *const *host_caches, const void *const *host_dra
       ptrs.cache[i] = host_caches[c0 + i];
       ptrs.draft[i] = host_drafts[c0 + i];
     }
-    dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(users), static_cast<unsigned>(n));
-    TTB_PAGE_UNITS(unit, U, TTB_CUDA(launchPdl(commitDraftKernel<U>, grid, dim3(PG_THREADS), 0, st, ptrs, static_cast<const int32_t *>(page_table),
+    // as many groups of caches as fill the GPU twice over (paths are often half as long as they may be)
+    const int64_t fill = 2 * smCount() * (2048 / PG_THREADS);
+    const int64_t groups = std::min<int64_t>(n, std::max<int64_t>(1, fill / (pieces * users)));
+    dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(users), static_cast<unsigned>(groups));
+    TTB_PAGE_UNITS(unit, U, TTB_CUDA(launchPdl(commitDraftKernel<U>, grid, dim3(PG_THREADS), 0, st, ptrs, n, static_cast<const int32_t *>(page_table),
                                                static_cast<const int32_t *>(cached_lens), static_cast<const int32_t *>(path),
                                                static_cast<const int32_t *>(path_lens), static_cast<int>(nodes), static_cast<int>(heads), blocks,
                                                static_cast<int>(block_size), static_cast<int>(pages), rowUnits, bad)))

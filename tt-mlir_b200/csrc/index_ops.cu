@@ -12,6 +12,8 @@
 // same on every run -- with all exchange distances below a tile done in shared memory.
 #include "common.cuh"
 
+#include <atomic>
+
 #include <cfloat>
 #include <type_traits>
 
@@ -366,7 +368,14 @@ static bool fillIdxDims(IdxDims &d, int rank, int dim, const int64_t *idxShape, 
 
 // Address of the current device's flag, for kernels of other files that skip a bad index.
 int indexBadFlag(int **flag) {
+  static std::atomic<int *> known[64]; // per device; asking the runtime costs about as much as a launch
+  int dev = 0;
+  TTB_CUDA(cudaGetDevice(&dev));
+  const bool kept = dev >= 0 && dev < 64;
+  *flag = kept ? known[dev].load(std::memory_order_acquire) : nullptr;
+  if (*flag) return TTB_OK;
   TTB_CUDA(cudaGetSymbolAddress(reinterpret_cast<void **>(flag), g_indexBad));
+  if (kept) known[dev].store(*flag, std::memory_order_release);
   return TTB_OK;
 }
 
