@@ -448,6 +448,112 @@ def test_sample_reads_rows_through_their_stride(kn):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_deep_cuts_under_a_few_heavy_tokens(kn, dtype):
+    """A few tokens, which a sample of the row hardly sees, hold most of the weight; top-k is deep, min-p lies on either
+    side of its border."""
+    gen = torch.Generator().manual_seed(31)
+    vocab, rows = 100003, 14
+    logits = torch.randn(rows, vocab, generator=gen) * 2.5
+    for r in range(rows):
+        logits[r, torch.randperm(vocab, generator=gen)[:24]] += torch.rand(24, generator=gen) * 12
+        logits[r, torch.randperm(vocab, generator=gen)[:1000]] = float("-inf")
+    k = [40000, 40000, 1501, 30000, 2000, 60000, 40000, 99999, 1600, 40000, 5000, 40000, 1400, 80000]
+    p = [1.0, 0.5, 0.9, 0.99, 1.0, 0.95, 1.0, 0.99, 0.999, 1.0, 0.7, 0.9, 0.99, 0.5]
+    heat = [1.0, 1.0, 0.8, 0.5, 0.5, 1.0, 0.6, 0.8, 0.5, 0.3, 1.0, 0.5, 0.7, 0.8]
+    low = [0.0, 0.0, 0.0, 0.0, 1e-6, 0.02, 1e-3, 0.0, 1e-4, 1e-12, 1e-7, 0.1, 0.0, 1e-9]
+    check_samples(kn, logits.to(dtype), torch.rand(rows, generator=gen).tolist(), heat, k, p, low)
+
+
+def test_sample_the_longest_rows(kn):
+    gen = torch.Generator().manual_seed(32)
+    logits = (torch.randn(4, 2 ** 22, generator=gen) * 2).to(torch.bfloat16)
+    logits[3, 2 ** 22 - 1] = 60.0
+    check_samples(kn, logits, [0.3, 0.8, 0.5, 0.5], heat=[0.5, 0.7, 0.0, 1.0], k=[50, 0, 0, 0], p=[1.0, 0.4, 1.0, 1.0])
+
+
+# ---- sizes and streams -----------------------------------------------------------------------------------------------------
+def test_caches_of_more_than_2_to_the_31_elements(kn):
+    """The last blocks of large caches give what the same blocks give in small ones; everything else holds NaN."""
+    gen = torch.Generator().manual_seed(41)
+    blocks, pages, Hkv, H, block, D, T = 33000, 34, 8, 16, 64, 128, 5
+    one = Hkv * block * D * 2
+    k, v = rand(gen, pages, Hkv, block, D), rand(gen, pages, Hkv, block, D)
+    big = []
+    for t in (k, v):
+        ptr = ctypes.c_void_p()
+        kn._check(kn.lib.ttb_malloc(ctypes.byref(ptr), ctypes.c_size_t(blocks * one), kn.stream))
+        kn._bufs.append(ptr)
+        kn._check(kn.lib.ttb_memset(ptr, 0xff, ctypes.c_size_t(blocks * one), kn.stream))
+        kn._check(kn.lib.ttb_memcpy_h2d(ctypes.c_void_p(ptr.value + (blocks - pages) * one), ctypes.c_void_p(t.data_ptr()), ctypes.c_size_t(pages * one),
+                                        kn.stream))
+        kn.sync()
+        big.append(ptr)
+    table = torch.randperm(pages, generator=gen)[None].to(torch.int32)
+    far = kn.up(table + (blocks - pages))
+    size = max(kn.lib.ttb_sdpa_window_decode_workspace_bytes(*kn.args(1, H, Hkv, D, pages * block, 10 ** 6, 0)),
+               kn.lib.ttb_sdpa_tree_workspace_bytes(*kn.args(1, T, H, Hkv, D, pages * block)), 16)
+    work, scale = kn.empty((size,), torch.uint8), 1 / math.sqrt(D)
+
+    n = 2150
+    q, pos = rand(gen, 1, 1, H, D), torch.tensor([n - 1], dtype=torch.int32)
+    out = kn.empty(q.shape, q.dtype)
+    kn.call("ttb_sdpa_window_decode", kn.up(q), *big, far, kn.up(pos), out, TAG[q.dtype], 1, H, Hkv, blocks, block, pages, D, 10 ** 6, 0, scale,
+            work, ctypes.c_size_t(size), kn.stream)
+    assert torch.equal(kn.download(out, q.shape, q.dtype), kn.decode(q, k, v, table, pos, 10 ** 6, 0))
+
+    q, kd, vd = rand(gen, 1, T, H, D), rand(gen, 1, T, Hkv, D), rand(gen, 1, T, Hkv, D)
+    lens, parents = torch.tensor([n], dtype=torch.int32), torch.tensor([[-1, 0, 0, 2, 1]], dtype=torch.int32)
+    out = kn.empty(q.shape, q.dtype)
+    kn.call("ttb_sdpa_tree", kn.up(q), kn.up(kd), kn.up(vd), *big, far, kn.up(lens), kn.up(parents), None, out, TAG[q.dtype], 1, T, H, Hkv, blocks, block,
+            pages, D, 1, 0, 0, scale, work, ctypes.c_size_t(size), kn.stream)
+    assert torch.equal(kn.download(out, q.shape, q.dtype), kn.tree(q, kd, vd, k, v, table, lens, parents))
+
+    arr, darr = (ctypes.c_void_p * 2)(*[b.value for b in big]), (ctypes.c_void_p * 2)(kn.up(kd).value, kn.up(vd).value)
+    path, count = torch.tensor([[0, 2, 3, 0, 0]], dtype=torch.int32), torch.tensor([3], dtype=torch.int32)
+    kn.call("ttb_paged_commit_draft", arr, darr, 2, far, kn.up(lens), kn.up(path), kn.up(count), TAG[q.dtype], 1, T, Hkv, blocks, block, pages, D, kn.stream)
+    last = int(table[0, n // block])
+    kn.call("ttb_paged_copy_blocks", arr, 2, kn.up(torch.tensor([[blocks - pages + last, 0]], dtype=torch.int32)), 1, TAG[q.dtype], blocks, Hkv, block, D,
+            kn.stream)
+    for ptr, t, d in zip(big, (k, v), (kd, vd)):
+        want = t[last].clone()
+        for i, node in enumerate((0, 2, 3)):
+            want[:, n % block + i] = d[0, node]
+        assert torch.equal(kn.download(ptr, want.shape, want.dtype), want)   # block 0, a copy of the one written
+    assert kn.bad() == 0
+
+
+def test_calls_on_two_streams_at_once(kn):
+    """Each stream with buffers and workspaces of its own: what they give alone."""
+    gen = torch.Generator().manual_seed(42)
+    H, Hkv, D, n, vocab = 8, 2, 128, 3000, 60000
+    other = ctypes.c_void_p()
+    kn._check(kn.lib.ttb_stream_create(ctypes.byref(other)))
+    jobs = []
+    for stream in (kn.stream, other):
+        logits, u, top_k = torch.randn(40, vocab, generator=gen) * 3, torch.rand(40, generator=gen), torch.randint(1, 20000, (40,), generator=gen).int()
+        q, kd, vd = rand(gen, 2, 6, H, D), rand(gen, 2, 6, Hkv, D), rand(gen, 2, 6, Hkv, D)
+        k, v, lens = rand(gen, 2, Hkv, n, D), rand(gen, 2, Hkv, n, D), torch.tensor([n, 1234], dtype=torch.int32)
+        parents = torch.tensor([[-1, 0, 1, 0, 3, 3]], dtype=torch.int32)
+        want = kn.sample(logits, u, None, top_k)[0], kn.tree(q, kd, vd, k, v, None, lens, parents)
+        size = kn.lib.ttb_sdpa_tree_workspace_bytes(*kn.args(2, 6, H, Hkv, D, n))
+        work, token, out = kn.empty((max(size, 16),), torch.uint8), kn.empty((40,), torch.int32), kn.empty(q.shape, q.dtype)
+        sample = (kn.up(logits), kn.up(u), None, kn.up(top_k), None, None, token, None, TAG[logits.dtype], 40, vocab, vocab, None, ctypes.c_size_t(0), stream)
+        tree = (kn.up(q), kn.up(kd), kn.up(vd), kn.up(k), kn.up(v), None, kn.up(lens), kn.up(parents), None, out, TAG[q.dtype], 2, 6, H, Hkv, 2, n, 1, D, 1, 0, 0,
+                1 / math.sqrt(D), work, ctypes.c_size_t(size), stream)
+        jobs.append((sample, tree, token, out, want))
+    for _ in range(5):
+        for sample, tree, *_ in jobs:
+            kn.call("ttb_sdpa_tree", *tree)
+            kn.call("ttb_sample_logits", *sample)
+    kn._check(kn.lib.ttb_stream_sync(other))
+    kn.sync()
+    for _, _, token, out, (want, want_out) in jobs:
+        assert torch.equal(kn.download(token, (40,), torch.int32), want)
+        assert torch.equal(kn.download(out, want_out.shape, want_out.dtype), want_out)
+    kn._check(kn.lib.ttb_stream_destroy(other))
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------
 def test_a_speculative_step(kn):
     """Draft tree -> attention -> logits -> greedy tokens -> accepted path -> cache -> next token's attention, and a fork."""
