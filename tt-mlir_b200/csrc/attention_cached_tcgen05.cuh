@@ -339,48 +339,51 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-    if (warp == 12 && lane == 0 && tiles > 0) {
+    const int rounds = __shfl_sync(0xffffffffu, tiles, 0);
+    if (warp == 12 && rounds > 0) { // the whole warp in step, see awMma
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmemBase, 0);
+      auto wait = [&](uint32_t bar, int parity, int where) { return __all_sync(0xffffffffu, mbarWait(bar, parity, abortP, where)) != 0; };
       constexpr uint32_t HIGH = (2u << 29) | (1u << 14) | (1024u >> 4); // as in the prompt kernel
       const uint32_t idS = instrDescF16(p.fmt, 128, 128, 0, 0), idPV = instrDescF16(p.fmt, 128, D, 0, 1);
       auto desc = [](uint32_t low) -> uint64_t { return (static_cast<uint64_t>(HIGH) << 32) | low; };
       const uint32_t qLow = sQ >> 4;
-      bool ok = mbarWait(qFull, 0, abortP, 4);
+      bool ok = wait(qFull, 0, 4);
       int stage = 0, phase = 0, old = 0, oldPhase = 0; // of tile j, of tile j - 2
-      for (int j = 0; ok && j < tiles + 2; ++j) {
+      for (int j = 0; ok && j < rounds + 2; ++j) {
         const int chain = j & 1;
-        const uint32_t sCol = tmemBase + chain * 128, oCol = tmemBase + 256 + chain * D;
+        const uint32_t sCol = tmem + chain * 128, oCol = tmem + 256 + chain * D;
         if (j >= 2) { // O += P V of the chain's tile before
           const uint32_t vLow = ((sRing + (2 * old + 1) * TILE) >> 4) | (static_cast<uint32_t>(COLS >> 4) << 16);
-          ok = mbarWait(full + 8 * (R + old), oldPhase, abortP, 8);
+          ok = wait(full + 8 * (R + old), oldPhase, 8);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            ok = ok && mbarWait(pReady + 16 * chain + 8 * h, ((j - 2) >> 1) & 1, abortP, 5);
+            ok = ok && wait(pReady + 16 * chain + 8 * h, ((j - 2) >> 1) & 1, 5);
             if (ok) {
               tcFenceAfter();
 #pragma unroll
-              for (int ks = 4 * h; ks < 4 * h + 4; ++ks) tcMmaTmemA(oCol, sCol + ks * 8, desc(vLow + ks * (2048 >> 4)), idPV, (j >= 4) | (ks > 0));
+              for (int ks = 4 * h; ks < 4 * h + 4; ++ks) awMmaTmemA(oCol, sCol + ks * 8, desc(vLow + ks * (2048 >> 4)), idPV, (j >= 4) | (ks > 0));
             }
           }
           if (!ok) break;
-          tcCommit(empty + 8 * (R + old));
-          if (j + 2 > tiles + 1) tcCommit(oFull + 8 * chain); // the chain's last tile
+          awCommit(empty + 8 * (R + old));
+          if (j + 2 > rounds + 1) awCommit(oFull + 8 * chain); // the chain's last tile
           if (++old == R) {
             old = 0;
             oldPhase ^= 1;
           }
         }
-        if (j < tiles) {
-          ok = mbarWait(full + 8 * stage, phase, abortP, 6);
+        if (j < rounds) {
+          ok = wait(full + 8 * stage, phase, 6);
           if (!ok) break;
           const uint32_t kLow = (sRing + 2 * stage * TILE) >> 4;
           tcFenceAfter();
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * COLS + (ks & 3) * 32) >> 4;
-            tcMma(sCol, desc(qLow + off), desc(kLow + off), idS, ks > 0);
+            awMma(sCol, desc(qLow + off), desc(kLow + off), idS, ks > 0);
           }
-          tcCommit(sFull + 8 * chain);
-          tcCommit(empty + 8 * stage);
+          awCommit(sFull + 8 * chain);
+          awCommit(empty + 8 * stage);
           if (++stage == R) {
             stage = 0;
             phase ^= 1;

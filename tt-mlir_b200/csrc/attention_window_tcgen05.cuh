@@ -109,6 +109,30 @@ __device__ __forceinline__ void awSoftmax(uint32_t (&sc)[4][32], uint32_t sAddr,
   l += (s0 + s1) + (s2 + s3);
 }
 
+// The products and their commits, called by a whole warp in step; one lane issues.  With the loop around them uniform the
+// descriptors can stay in uniform registers (issued from a branch that one lane takes: 567 us instead of 538 for the
+// prompt below, from a warm L2).
+__device__ __forceinline__ void awMma(uint32_t tmemD, uint64_t descA, uint64_t descB, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, one;\n\t"
+               "elect.sync _|one, 0xffffffff;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(tmemD), "l"(descA), "l"(descB), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void awMmaTmemA(uint32_t tmemD, uint32_t tmemA, uint64_t descB, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, one;\n\t"
+               "elect.sync _|one, 0xffffffff;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(tmemD), "r"(tmemA), "l"(descB), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void awCommit(uint32_t bar) {
+  asm volatile("{\n\t.reg .pred one;\n\t"
+               "elect.sync _|one, 0xffffffff;\n\t"
+               "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+               ::"r"(bar) : "memory");
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(AW_THREADS, 1)
     sdpaWindowTcgen05Kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
@@ -218,15 +242,18 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
         }
       }
     } else if (warp == 1) {
-      if (lane == 0 && tiles > 0) {
-        // One thread issues everything, and 32 products per pair of row tiles and key tile leave it 64 cycles each: the
-        // operand descriptors differ only in the address field of their low word, so each costs one addition (computed in
-        // full for every product, the issuing thread took 3300 cycles per key tile and set the pace).
+      const int rounds = __shfl_sync(0xffffffffu, tiles, 0);
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmemBase, 0);
+      auto wait = [&](uint32_t bar, int parity, int where) { return __all_sync(0xffffffffu, mbarWait(bar, parity, abortP, where)) != 0; };
+      if (rounds > 0) {
+        // 32 products per pair of row tiles and key tile leave the issuing lane 64 cycles each: the operand descriptors
+        // differ only in the address field of their low word, so each costs one addition (computed in full for every
+        // product, the lane took 3300 cycles per key tile and set the pace).
         constexpr uint32_t IDV = (2u << 29) | (1u << 14) | (1024u >> 4); // high word: 128-byte swizzle, version, 1024 bytes per 8 rows
         const uint32_t idS = instrDescF16(p.fmt, 128, AW_KEYS, 0, 0), idPV = instrDescF16(p.fmt, 128, D, 0, 1);
         auto desc = [](uint32_t low) -> uint64_t { return (static_cast<uint64_t>(IDV) << 32) | low; };
         const uint32_t qLow = sQ >> 4, ringLow = sRing >> 4, apart = static_cast<uint32_t>(COLS >> 4) << 16; // V: distance of its 64-column parts
-        bool ok = mbarWait(qFull, 0, abortP, 3);
+        bool ok = wait(qFull, 0, 3);
         int slot = 0, phase = 0; // of the next tile in the ring
         auto advance = [&] {
           if (++slot == R) {
@@ -234,46 +261,46 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
             phase ^= 1;
           }
         };
-        for (int j = 0; ok && j <= tiles; ++j) {
+        for (int j = 0; ok && j <= rounds; ++j) {
           // the ring holds V_{j-1} (from the second round on), then K_j
           const int vSlot = slot;
           if (j > 0) {
-            ok = mbarWait(full + 8 * slot, phase, abortP, 5);
-            if (ok && j == tiles && clean) ok = mbarWait(vClean, 0, abortP, 6);
+            ok = wait(full + 8 * slot, phase, 5);
+            if (ok && j == rounds && clean) ok = wait(vClean, 0, 6);
             advance();
           }
           const int kSlot = slot;
-          if (ok && j < tiles) {
-            ok = mbarWait(full + 8 * slot, phase, abortP, 4);
+          if (ok && j < rounds) {
+            ok = wait(full + 8 * slot, phase, 4);
             advance();
           }
           const uint32_t vLow = (ringLow + vSlot * (TILE >> 4)) | apart, kLow = ringLow + kSlot * (TILE >> 4);
           for (int m = 0; ok && m < tilesM; ++m) {
-            const uint32_t sCol = tmemBase + m * AW_KEYS, oCol = tmemBase + 2 * AW_KEYS + m * D;
+            const uint32_t sCol = tmem + m * AW_KEYS, oCol = tmem + 2 * AW_KEYS + m * D;
             if (j > 0) { // O_m += P_m V: steps of 16 keys as each half of the probabilities arrives; P from tensor memory, V MN-major
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                ok = ok && mbarWait(pReady + 16 * m + 8 * h, (j - 1) & 1, abortP, 7);
+                ok = ok && wait(pReady + 16 * m + 8 * h, (j - 1) & 1, 7);
                 if (ok) {
                   tcFenceAfter();
 #pragma unroll
-                  for (int ks = 4 * h; ks < 4 * h + 4; ++ks) tcMmaTmemA(oCol, sCol + ks * 8, desc(vLow + ks * (2048 >> 4)), idPV, (j > 1) | (ks > 0));
+                  for (int ks = 4 * h; ks < 4 * h + 4; ++ks) awMmaTmemA(oCol, sCol + ks * 8, desc(vLow + ks * (2048 >> 4)), idPV, (j > 1) | (ks > 0));
                 }
               }
               if (!ok) break;
-              if (m == tilesM - 1) tcCommit(empty + 8 * vSlot);
-              if (j == tiles) tcCommit(oFull + 8 * m);
+              if (m == tilesM - 1) awCommit(empty + 8 * vSlot);
+              if (j == rounds) awCommit(oFull + 8 * m);
             }
-            if (j < tiles) { // S_m = Q_m K^T: steps of 16 along d, both operands K-major
+            if (j < rounds) { // S_m = Q_m K^T: steps of 16 along d, both operands K-major
               const uint32_t aLow = qLow + m * (TILE >> 4);
               tcFenceAfter();
 #pragma unroll
               for (int ks = 0; ks < D / 16; ++ks) {
                 const uint32_t off = ((ks >> 2) * COLS + (ks & 3) * 32) >> 4;
-                tcMma(sCol, desc(aLow + off), desc(kLow + off), idS, ks > 0);
+                awMma(sCol, desc(aLow + off), desc(kLow + off), idS, ks > 0);
               }
-              tcCommit(sFull + 8 * m);
-              if (m == tilesM - 1) tcCommit(empty + 8 * kSlot);
+              awCommit(sFull + 8 * m);
+              if (m == tilesM - 1) awCommit(empty + 8 * kSlot);
             }
           }
         }
