@@ -365,7 +365,8 @@ TTB_API int ttb_sdpa_decode_paged(const void *q, const void *k, const void *v, c
  * position p sees the keys j <= p with j < sinks or j > p - window: the last `window` positions, its own included, and the
  * first `sinks` ones ("attention sinks").  out = softmax(scale q k^T) v over the keys seen, f32 inside, probabilities
  * rounded to `dtype` for the second product, the result rounded once; a row that sees no key is zero.  Keys and values
- * that no row of the call sees are not read, whatever they hold.  No workspace may be shared by calls that can overlap
+ * that no row of the call sees are not read, whatever they hold; a NaN or an infinity in a value that one row sees may
+ * show in other rows of the call.  No workspace may be shared by calls that can overlap
  * on the GPU (two streams, or two captured graphs replayed at the same time).
  *   ttb_sdpa_window         a prompt, or the chunk of one that starts at position `offset`: query row r is the token at
  *                           r + offset.  q, out [batch, heads_q, seq_q, head_dim], k, v [batch, heads_kv, seq_kv, head_dim];
@@ -469,7 +470,8 @@ TTB_API int ttb_sampling(const void *values, const void *indices, const void *k,
  *   uniform      in [0, 1): the token is the first index, in the vocabulary's order, at which the running sum of the weights
  *                that stayed exceeds uniform * their total
  * out (Int32 [rows]) gets the token and prob (f32 [rows], nullable) its share of the weights that stayed.  -inf and NaN
- * logits are never taken; a row of nothing else gives -1 and 0.  The same inputs give the same token on every run.
+ * logits are never taken; a row of nothing else gives -1 and 0.  A weight below 2^-60 of the row's largest counts as
+ * none.  vocab is limited to 2^22.  The same inputs give the same token on every run.
  * `workspace`: ttb_sample_logits_workspace_bytes(...), not shared by calls that can overlap on the GPU.
  * ttb_sampling draws among pre-selected candidates with its own generator (operations/reduction/sampling.cpp). */
 TTB_API size_t ttb_sample_logits_workspace_bytes(int64_t rows, int64_t vocab);
