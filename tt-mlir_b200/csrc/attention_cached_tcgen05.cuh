@@ -12,6 +12,10 @@
 // Even and odd tiles are two chains of their own (scores, probabilities, output and maximum), so that one chain's softmax
 // runs beside the other's products; at the end the odd chain hands its output to the even one through the ring's memory.
 // Bound: HBM as long as a tile of keys and values (64 KB at head_dim 128) takes longer to arrive than a chain's round trip.
+// Measured (16 users x 31 nodes, 32 query / 8 kv heads x 128, up to 8192 cached tokens in blocks of 64, bf16): 104 us, 62 %
+// of the measured HBM rate over the users' own lengths; 128 CTAs on 148 SMs, the longest user sets the time.  Steps: one
+// chain 261 (mma.sync), two chains 159, TMA boxes 114, keys and values fetched apart and joined in the CTA 100; two, three
+// or four splits per user 118, 129, 133.
 #pragma once
 
 #include "attention_cached.cuh"

@@ -16,6 +16,8 @@
 // tile into WM groups of rows and 4 / WM groups of keys, each with its own running maximum and sum, merged at the
 // end through shared memory.  One row tile per kv head is bound by HBM (16 rows: 16 multiply-adds per byte read).
 // With few users the slots are split over `splits` CTAs and a second kernel joins the parts.
+// Measured: one token for each of 64 users, 32 query / 8 kv heads x 128, window 4096, 16 sinks, bf16: 192 us, 85 % of the
+// measured HBM rate; one user, 8 heads x 64, window 1000: 12 us, of which a launch that does nothing takes 8.
 #include "attention_cached.cuh"
 #include "common.cuh"
 

@@ -17,13 +17,14 @@
 // just two barriers per tile and step (scores there; probabilities there).
 //   TMEM: S_A 0..127, S_B 128..255, O_A 256.., O_B 256 + D..
 //   Shared memory: Q_A | Q_B | ring of K / V tiles | barriers.
-// Measured (32 query / 8 kv heads x 16384 tokens, head_dim 128, window 2048, 64 sinks, bf16): 0.62 ms, 0.86 PFLOP/s, 51 %
-// of the measured cuBLAS rate.  With parts switched off: without exponentials, maxima and sums 0.54 ms, without the
-// products 0.46 ms, without either (loads, tensor-memory traffic, barriers) 0.33 ms, without the TMA loads unchanged.  So
-// neither unit is saturated (43 % of the cycles each): a row tile's chain of scores, hand-over, softmax, hand-over, values
-// is what it waits for, and two row tiles (tensor memory holds no more) overlap only part of it.  Tried and slower: two
-// threads per row with their maxima exchanged (1.35 ms, 96 registers per thread spill), exponentials ahead of the maximum
-// (0.76 ms, spills again).
+// Measured (32 query / 8 kv heads x 16384 tokens, head_dim 128, window 2048, 64 sinks, bf16): 0.605 ms, 0.88 PFLOP/s, 52 %
+// of the measured cuBLAS rate (0.54 ms from a warm L2).  With parts switched off, at 0.62 ms: without exponentials, maxima
+// and sums 0.54, without the products 0.46, without either (loads, tensor-memory traffic, barriers) 0.33, without the TMA
+// loads unchanged.  So neither unit is saturated (the tensor pipe works 48 % of the cycles): a row tile's chain of scores,
+// hand-over, softmax, hand-over, values is what it waits for, and two row tiles (tensor memory holds no more) overlap only
+// part of it.  Tried and slower: two threads per row with their maxima exchanged (1.35 ms, 96 registers per thread spill),
+// exponentials ahead of the maximum (0.76 ms, spills again), hand-overs of 64 keys (0.63 from a warm L2: the score products
+// become N = 64); three eighths of the exponentials as polynomials gained less than 1 %.
 #pragma once
 
 namespace ttb {
