@@ -333,6 +333,45 @@ def test_commit_draft_leaves_out_rows_without_a_place(kn):
     assert torch.equal(got, t) and kn.bad() == 1
 
 
+def test_commit_draft_of_many_users(kn):
+    """More users and pieces than fill the GPU: every CTA serves all caches in turn."""
+    gen = torch.Generator().manual_seed(51)
+    users, nodes, heads, block, dim, caches = 1200, 33, 8, 8, 64, 3
+    pages = 6
+    blocks = users * pages
+    table = torch.randperm(blocks, generator=gen).view(users, pages).to(torch.int32)
+    lens = torch.randint(0, pages * block - nodes + 1, (users,), generator=gen).to(torch.int32)
+    count = torch.randint(0, nodes + 1, (users,), generator=gen).to(torch.int32)
+    path = torch.stack([torch.randperm(nodes, generator=gen) for _ in range(users)]).to(torch.int32)
+    before = [torch.randint(-128, 128, (blocks, heads, block, dim), generator=gen, dtype=torch.int8) for _ in range(caches)]
+    drafts = [torch.randint(-128, 128, (users, nodes, heads, dim), generator=gen, dtype=torch.int8) for _ in range(caches)]
+    got = kn.commit(before, drafts, table, lens, path, count)
+    who = torch.arange(users)[:, None].expand(users, nodes)
+    step = torch.arange(nodes)[None].expand(users, nodes)
+    live = step < count[:, None]
+    at = lens[:, None].long() + step
+    who, node, at = who[live], path[live].long(), at[live]
+    for b, d, g in zip(before, drafts, got):
+        want = b.clone()
+        want[table[who, at // block].long(), :, at % block] = d[who, node]
+        assert torch.equal(g, want)
+    assert kn.bad() == 0
+
+
+def test_more_caches_than_a_launch_takes(kn):
+    gen = torch.Generator().manual_seed(52)
+    caches = [torch.randint(-128, 128, (4, 1, 2, 16), generator=gen, dtype=torch.int8) for _ in range(259)]
+    drafts = [torch.randint(-128, 128, (1, 2, 1, 16), generator=gen, dtype=torch.int8) for _ in range(259)]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    for c, g in zip(caches, kn.copy_blocks(caches, i32([1, 3], [1, 0]))):
+        assert torch.equal(g, c[[1, 1, 2, 1]])
+    for c, d, g in zip(caches, drafts, kn.commit(caches, drafts, i32([2, 0]), i32(1), i32([1, 0]), i32(2))):
+        want = c.clone()
+        want[2, 0, 1], want[0, 0, 0] = d[0, 1, 0], d[0, 0, 0]
+        assert torch.equal(g, want)
+    assert kn.bad() == 0
+
+
 # ---- sampling -----------------------------------------------------------------------------------------------------------
 def check_samples(kn, logits, u, heat=None, k=None, p=None, low=None):
     rows = logits.shape[0]
@@ -470,6 +509,12 @@ def test_sample_the_longest_rows(kn):
     logits = (torch.randn(4, 2 ** 22, generator=gen) * 2).to(torch.bfloat16)
     logits[3, 2 ** 22 - 1] = 60.0
     check_samples(kn, logits, [0.3, 0.8, 0.5, 0.5], heat=[0.5, 0.7, 0.0, 1.0], k=[50, 0, 0, 0], p=[1.0, 0.4, 1.0, 1.0])
+
+
+def test_sample_many_short_rows(kn):
+    logits = torch.randn(70001, 5, generator=torch.Generator().manual_seed(53))
+    token, prob = kn.sample(logits, torch.zeros(70001), torch.zeros(70001))
+    assert torch.equal(token.long(), logits.argmax(dim=1)) and bool((prob == 1).all())
 
 
 # ---- sizes and streams -----------------------------------------------------------------------------------------------------
