@@ -15,7 +15,8 @@
 // touched.  A CTA walks its run of slots in tiles of 64 through a ring of cp.async stages; the four warps split a
 // tile into WM groups of rows and 4 / WM groups of keys, each with its own running maximum and sum, merged at the
 // end through shared memory.  One row tile per kv head is bound by HBM (16 rows: 16 multiply-adds per byte read).
-// With few users the slots are split over `splits` CTAs and a second kernel joins the parts.
+// With few users the slots are split over `splits` CTAs: up to 8 are a cluster and join their parts through its shared
+// memory, parts of more go through the workspace and a second kernel.
 // Measured: one token for each of 64 users, 32 query / 8 kv heads x 128, window 4096, 16 sinks, bf16: 192 us, 85 % of the
 // measured HBM rate; one user, 8 heads x 64, window 1000: 12 us, of which a launch that does nothing takes 8.
 #include "attention_cached.cuh"
@@ -29,6 +30,7 @@ namespace ttb {
 constexpr int WN_THREADS = 128;
 constexpr int WN_KT = 64;    // slots per tile
 constexpr int WN_NODES = 64; // most nodes of a tree (one 64-bit mask per node)
+constexpr int WN_CLUSTER = 8; // CTAs of a cluster that every GPU of this kind takes
 
 enum WindowMode { kPrompt = 0, kDecode = 1, kTree = 2 };
 
@@ -43,7 +45,7 @@ struct WindowParams {
   int batch, nq, heads, kvHeads, G, keys; // keys: most cached positions of a user
   int offset, window, sinks, splits, mode;
   float scaleLog2;                        // scale * log2(e)
-  float *pm, *pl, *po;                    // partial results of the splits
+  float *pm, *pl, *po;                    // partial results of the splits, when there are more than a cluster's
 };
 
 __device__ __forceinline__ uint32_t wnSmem(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -113,6 +115,7 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
   __shared__ unsigned long long line[WN_NODES];                  // bit u of line[t]: node u is t or an ancestor of t
   __shared__ int up[WN_NODES];
   __shared__ float partM[4][16], partL[4][16];
+  __shared__ float rowM[BM], rowL[BM];                           // of all key groups, for the cluster
   pdlLaunchDependents();
   pdlWait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane >> 2, t4 = lane & 3;
@@ -386,6 +389,7 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
   }
   __syncthreads();
   const int liveRows = p.mode == kTree ? draft * p.G : rows;
+  const bool clustered = p.splits > 1 && p.splits <= WN_CLUSTER;
   for (int i = tid; i < BM * (D / 4); i += WN_THREADS) {
     const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
     if (row >= liveRows) continue;
@@ -407,7 +411,13 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
       acc.w = fmaf(x.w, f, acc.w);
     }
     const int head = kvh * p.G + row % p.G, qi = row / p.G;
-    if (p.splits > 1) {
+    if (clustered) { // over the first group's part, which only this thread reads
+      *reinterpret_cast<float4 *>(xo + static_cast<size_t>(r) * D + d) = acc;
+      if (d == 0) {
+        rowM[r] = mx;
+        rowL[r] = den;
+      }
+    } else if (p.splits > 1) {
       const int64_t part = ((static_cast<int64_t>(b) * p.nq + qi) * p.heads + head) * p.splits + split;
       *reinterpret_cast<float4 *>(p.po + part * D + d) = acc;
       if (d == 0) {
@@ -422,6 +432,48 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
       *reinterpret_cast<uint2 *>(out + b * p.ob + head * p.oh + qi * p.os + d) = w;
     }
   }
+  if (!clustered) return;
+  // ---- join the cluster's parts: its CTAs share the elements out
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  auto remote = [](const void *at, int rank) { // the same place in another CTA
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(wnSmem(at)), "r"(rank));
+    return a;
+  };
+  for (int i = tid + split * WN_THREADS; i < BM * (D / 4); i += WN_THREADS * p.splits) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
+    if (row >= liveRows) continue;
+    float ms[WN_CLUSTER], mx = -INFINITY, den = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < WN_CLUSTER; ++c) {
+      ms[c] = -INFINITY;
+      if (c < p.splits) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[c]) : "r"(remote(&rowM[r], c)));
+      mx = fmaxf(mx, ms[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < WN_CLUSTER; ++c) {
+      if (ms[c] == -INFINITY) continue; // this part saw nothing of the row
+      const float f = exp2f(ms[c] - mx);
+      float4 x;
+      float part;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote(&rowL[r], c)));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(remote(xo + static_cast<size_t>(r) * D + d, c)));
+      den += part * f;
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
+    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+    uint2 w;
+    w.x = wnPack<T>(acc.x * inv, acc.y * inv);
+    w.y = wnPack<T>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2 *>(out + b * p.ob + (kvh * p.G + row % p.G) * p.oh + (row / p.G) * p.os + d) = w;
+  }
+  // no CTA leaves while another may still read its memory
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Joins the splits of a row: one warp per row of [batch, nq, heads], each lane four dims at a time.
@@ -594,11 +646,24 @@ static int launchWindowMma(const void *q, const void *k, const void *v, const vo
   const int64_t mts = (static_cast<int64_t>(p.nq) * p.G + BM - 1) / BM;
   TTB_CHECK(mts * p.splits <= 0x7fffffff, "too many query rows");
   dim3 grid(static_cast<unsigned>(mts * p.splits), static_cast<unsigned>(p.kvHeads), static_cast<unsigned>(p.batch));
-  TTB_CUDA(launchPdl(windowMmaKernel<T, D, WM>, grid, dim3(WN_THREADS), smem, st, static_cast<const T *>(q), static_cast<const T *>(k),
-                     static_cast<const T *>(v), static_cast<const T *>(kd), static_cast<const T *>(vd), static_cast<T *>(out), p));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(WN_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits <= WN_CLUSTER ? p.splits : 1; // the splits of a row tile are neighbours
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdlEnabled() ? 2 : 1;
+  TTB_CUDA(cudaLaunchKernelEx(&cfg, windowMmaKernel<T, D, WM>, static_cast<const T *>(q), static_cast<const T *>(k), static_cast<const T *>(v),
+                              static_cast<const T *>(kd), static_cast<const T *>(vd), static_cast<T *>(out), p));
   countLaunch();
   TTB_LAUNCH_CHECK();
-  return p.splits > 1 ? launchWindowJoin<T, D>(out, p, st) : TTB_OK;
+  return p.splits > WN_CLUSTER ? launchWindowJoin<T, D>(out, p, st) : TTB_OK;
 }
 
 template <typename T, int D>
