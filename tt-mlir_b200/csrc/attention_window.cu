@@ -581,7 +581,11 @@ static int windowSplits(int64_t batch, int64_t kvHeads, int64_t rows, int64_t ma
   const int64_t bm = 16 * windowRowTile(rows);
   const int64_t base = batch * kvHeads * ((rows + bm - 1) / bm);
   const int64_t want = (2 * smCount() + base - 1) / base, most = (maxSlots + 127) / 128;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, 128})));
+  const int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, 128})));
+  // A cluster's join costs less than a second kernel and its round trip through memory, as long as each of its CTAs has no
+  // more than some 512 slots.  Measured, one user, 32 query / 8 kv heads x 128, one cluster of 8 / all splits and a second
+  // kernel, us: 1100 slots 14 / 17, 2000 15 / 20, 2500 16 / 22, 4000 21 / 26.
+  return splits > WN_CLUSTER && maxSlots <= 4096 ? WN_CLUSTER : splits;
 }
 
 // How a tree's rows are computed, from the sizes that its workspace is asked for with.
@@ -614,8 +618,9 @@ static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kv
   return t;
 }
 
-static size_t windowPartBytes(int64_t batch, int64_t nq, int64_t heads, int64_t dim, int64_t splits) {
-  if (splits <= 1) return 0;
+// Partial results in the workspace: none for up to `joined` splits.
+static size_t windowPartBytes(int64_t batch, int64_t nq, int64_t heads, int64_t dim, int64_t splits, int joined) {
+  if (splits <= joined) return 0;
   return static_cast<size_t>(batch) * nq * heads * splits * (dim + 2) * sizeof(float);
 }
 
@@ -812,7 +817,7 @@ int ttb_sdpa_window(const void *q, const void *k, const void *v, const void *kv_
 size_t ttb_sdpa_window_decode_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t positions, int64_t window,
                                               int64_t sinks) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || positions <= 0 || heads % kv_heads) return 0;
-  return windowPartBytes(batch, 1, heads, head_dim, windowSplits(batch, kv_heads, heads / kv_heads, maxVisible(positions, window, sinks)));
+  return windowPartBytes(batch, 1, heads, head_dim, windowSplits(batch, kv_heads, heads / kv_heads, maxVisible(positions, window, sinks)), WN_CLUSTER);
 }
 
 int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const void *page_table, const void *cur_pos, void *out, int dtype,
@@ -833,7 +838,7 @@ int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const vo
   p.qh = p.oh = head_dim;
   const int64_t slots = maxVisible(positions, window, sinks);
   p.splits = windowSplits(batch, kv_heads, p.G, slots);
-  const size_t need = windowPartBytes(batch, 1, heads, head_dim, p.splits);
+  const size_t need = windowPartBytes(batch, 1, heads, head_dim, p.splits, WN_CLUSTER);
   TTB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (see ttb_sdpa_window_decode_workspace_bytes)");
   const int64_t parts = static_cast<int64_t>(batch) * heads * p.splits;
   p.po = static_cast<float *>(workspace);
@@ -848,7 +853,8 @@ int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const vo
 
 size_t ttb_sdpa_tree_workspace_bytes(int batch, int nodes, int heads, int kv_heads, int head_dim, int64_t positions) {
   if (batch <= 0 || nodes <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || positions <= 0 || heads % kv_heads) return 0;
-  return windowPartBytes(batch, nodes, heads, head_dim, treePlan(batch, nodes, heads, kv_heads, head_dim, positions).splits);
+  const TreePlan plan = treePlan(batch, nodes, heads, kv_heads, head_dim, positions);
+  return windowPartBytes(batch, nodes, heads, head_dim, plan.splits, plan.tall ? 1 : WN_CLUSTER);
 }
 
 int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const void *k_cache, const void *v_cache, const void *page_table,
@@ -878,7 +884,7 @@ int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const
   // The workspace must not depend on the window (its size is asked for without one), so neither do the splits.
   const TreePlan plan = treePlan(batch, nodes, heads, kv_heads, head_dim, positions);
   p.splits = plan.splits;
-  const size_t need = windowPartBytes(batch, nodes, heads, head_dim, p.splits);
+  const size_t need = windowPartBytes(batch, nodes, heads, head_dim, p.splits, plan.tall ? 1 : WN_CLUSTER);
   TTB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (see ttb_sdpa_tree_workspace_bytes)");
   const int flagged = indexBadFlag(&p.bad);
   if (flagged) return flagged;
