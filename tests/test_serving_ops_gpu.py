@@ -208,6 +208,7 @@ def test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts,
     assert kn.bad() == 0
 
 
+@pytest.mark.parametrize("room", [2304, 4352])
 @pytest.mark.parametrize("dtype,H,Hkv,D,block,lens,T,kind,window,sinks,drafts,shared", [
     (torch.bfloat16, 8, 2, 128, 32, [100, 0, 1, 2300], 1, "star", 0, 0, None, False),
     (torch.float16, 4, 4, 64, 24, [333, 5, 2200], 13, "random", 50, 4, [13, 6, 0], False),
@@ -217,8 +218,13 @@ def test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts,
     (torch.bfloat16, 32, 4, 128, 64, [2303, 513], 33, "star", 100, 0, None, False),
     (torch.bfloat16, 8, 8, 64, 128, [2048, 127, 128], 5, "random", 1500, 33, None, False),
     (torch.float16, 8, 1, 128, 40, [2280], 40, "random", 10 ** 12, 2, [33], False)])
-def test_tree_in_a_large_cache(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared):
-    test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared, room=2304)
+def test_tree_in_a_large_cache(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared, room):
+    test_tree(kn, dtype, H, Hkv, D, block, lens, T, kind, window, sinks, drafts, shared, room=room)
+
+
+def test_tree_of_many_users_in_a_middling_cache(kn):
+    lens = torch.randint(0, 2100, (40,), generator=torch.Generator().manual_seed(61)).tolist()
+    test_tree(kn, torch.bfloat16, 8, 2, 64, 32, lens, 9, "random", 0, 0, None, False, room=2304)
 
 
 def test_tree_reports_a_parent_that_is_not_an_earlier_node(kn):
@@ -521,7 +527,7 @@ def test_sample_many_short_rows(kn):
 def test_caches_of_more_than_2_to_the_31_elements(kn):
     """The last blocks of large caches give what the same blocks give in small ones; everything else holds NaN."""
     gen = torch.Generator().manual_seed(41)
-    blocks, pages, Hkv, H, block, D, T = 33000, 34, 8, 16, 64, 128, 5
+    blocks, pages, Hkv, H, block, D, T = 33000, 68, 8, 16, 64, 128, 5
     one = Hkv * block * D * 2
     k, v = rand(gen, pages, Hkv, block, D), rand(gen, pages, Hkv, block, D)
     big = []
@@ -540,7 +546,7 @@ def test_caches_of_more_than_2_to_the_31_elements(kn):
                kn.lib.ttb_sdpa_tree_workspace_bytes(*kn.args(1, T, H, Hkv, D, pages * block)), 16)
     work, scale = kn.empty((size,), torch.uint8), 1 / math.sqrt(D)
 
-    n = 2150
+    n = 4310
     q, pos = rand(gen, 1, 1, H, D), torch.tensor([n - 1], dtype=torch.int32)
     out = kn.empty(q.shape, q.dtype)
     kn.call("ttb_sdpa_window_decode", kn.up(q), *big, far, kn.up(pos), out, TAG[q.dtype], 1, H, Hkv, blocks, block, pages, D, 10 ** 6, 0, scale,
@@ -571,7 +577,7 @@ def test_caches_of_more_than_2_to_the_31_elements(kn):
 def test_calls_on_two_streams_at_once(kn):
     """Each stream with buffers and workspaces of its own: what they give alone."""
     gen = torch.Generator().manual_seed(42)
-    H, Hkv, D, n, vocab = 8, 2, 128, 3000, 60000
+    H, Hkv, D, n, vocab = 8, 2, 128, 5000, 60000
     other = ctypes.c_void_p()
     kn._check(kn.lib.ttb_stream_create(ctypes.byref(other)))
     jobs = []

@@ -18,7 +18,7 @@
 // With few users the slots are split over `splits` CTAs: up to 8 are a cluster and join their parts through its shared
 // memory, parts of more go through the workspace and a second kernel.
 // Measured: one token for each of 64 users, 32 query / 8 kv heads x 128, window 4096, 16 sinks, bf16: 192 us, 85 % of the
-// measured HBM rate; one user, 8 heads x 64, window 1000: 12 us, of which a launch that does nothing takes 8.
+// measured HBM rate; one user, 8 heads x 64, window 1000: 10 us, of which a launch that does nothing takes 8.
 #include "attention_cached.cuh"
 #include "common.cuh"
 
@@ -596,10 +596,11 @@ struct TreePlan {
 static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kvHeads, int64_t dim, int64_t positions) {
   const int64_t rows = nodes * (heads / kvHeads), slots = positions + nodes;
   TreePlan t;
-  // The tensor-core kernel reads faster but starts slower (128 KB of ring to fill, tensor memory to claim).  Measured with
-  // 8 kv heads x 4, head_dim 128, this kernel / that one, us: 1 user, 1000 tokens, 4 .. 32 nodes: 19 .. 26 / 27 .. 32;
-  // 4 users, 4000 tokens, 8 nodes: 42 / 36; 16 users, 8192 tokens, 4 nodes: 120 / 107, 16 nodes: 177 / 109.
-  t.tall = slots >= 2048 && (dim == 64 || dim == 128);
+  // The tensor-core kernel reads faster but starts slower (128 KB of ring to fill, tensor memory to claim, a second kernel
+  // for the join).  Measured with 8 kv heads x 4, head_dim 128, this kernel / that one, us: 1 user, 2500 tokens, 8 nodes
+  // 29 / 21, 4000 tokens, 8 .. 32 nodes 30 .. 36 / 23 .. 35, 7000 tokens 35 / 40; 4 users, 4000 tokens, 8 nodes 36 / 30; 16
+  // users, 2500 tokens, 8 nodes 49 / 61, 8192 tokens, 4 nodes 107 / 120, 16 nodes 109 / 177.
+  t.tall = (dim == 64 || dim == 128) && (slots > 4096 || (slots >= 2048 && 2 * batch * kvHeads > smCount()));
   if (!t.tall) {
     t.splits = windowSplits(batch, kvHeads, rows, slots);
     return t;
