@@ -364,10 +364,10 @@ TTB_API int ttb_sdpa_decode_paged(const void *q, const void *k, const void *v, c
 /* Attention inside a sliding window, and of a few rows over a long cache (csrc/attention_window.cu).  The token at
  * position p sees the keys j <= p with j < sinks or j > p - window: the last `window` positions, its own included, and the
  * first `sinks` ones ("attention sinks").  out = softmax(scale q k^T) v over the keys seen, f32 inside, probabilities
- * rounded to `dtype` for the second product, the result rounded once; a row that sees no key is zero.  Keys and values
- * that no row of the call sees are not read, whatever they hold; a NaN or an infinity in a value that one row sees may
- * show in other rows of the call.  No workspace may be shared by calls that can overlap
- * on the GPU (two streams, or two captured graphs replayed at the same time).
+ * rounded to `dtype` for the second product, the result rounded once; a row that sees no key is zero, a row with a NaN among
+ * its scores is NaN (and no other row for it).  Keys and values that no row of the call sees are not read, whatever they
+ * hold; a NaN or an infinity in a value that one row sees may show in other rows of the call.  No workspace may be shared by
+ * calls that can overlap on the GPU (two streams, or two captured graphs replayed at the same time).
  *   ttb_sdpa_window         a prompt, or the chunk of one that starts at position `offset`: query row r is the token at
  *                           r + offset.  q, out [batch, heads_q, seq_q, head_dim], k, v [batch, heads_kv, seq_kv, head_dim];
  *                           the *_strides3 are host arrays of element strides {batch, head, seq} (null: dense; head_dim is

@@ -293,14 +293,14 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
         asm volatile("ld.shared.b32 %0, [%1];" : "=f"(ref1) : "r"(slot + D * 512));
         asm volatile("ld.shared.b32 %0, [%1];" : "=f"(l1) : "r"(slot + (D + 1) * 512));
         const float both = fmaxf(ref, ref1);
-        f0 = ref == -INFINITY ? 0.0f : fastExp2((ref - both) * sl2);
-        f1 = ref1 == -INFINITY ? 0.0f : fastExp2((ref1 - both) * sl2);
+        f0 = l == 0.0f ? 0.0f : fastExp2((ref - both) * sl2);
+        f1 = l1 == 0.0f ? 0.0f : fastExp2((ref1 - both) * sl2);
         l = l * f0 + l1 * f1;
         ref = both;
       }
       const bool live = ok && row < draft * p.G;
       const int64_t orow = (static_cast<int64_t>(b) * p.nq + row / p.G) * p.heads + kvh * p.G + row % p.G, part = orow * p.splits + split;
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (l > 0.0f) {
+            if (l != 0.0f) { // a NaN among them
               w.x = packPair<T>(x[g * 8] * inv, x[g * 8 + 1] * inv);
               w.y = packPair<T>(x[g * 8 + 2] * inv, x[g * 8 + 3] * inv);
               w.z = packPair<T>(x[g * 8 + 4] * inv, x[g * 8 + 5] * inv);

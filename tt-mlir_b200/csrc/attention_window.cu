@@ -7,7 +7,9 @@
 // out = softmax(scale q k^T) v over the keys that a row sees: key j is seen when j <= p and (j < sinks or
 // j > p - window); of the drafted keys a node sees its own and its ancestors', inside the same window.  Scores,
 // maxima, sums and the output accumulate in f32; the probabilities are rounded to the operands' type for the second
-// contraction (their sum is taken before that rounding), the result is rounded once.  A row that sees no key is zero.
+// contraction (their sum is taken before that rounding), the result is rounded once.  A row that sees no key is zero; one
+// that sees a NaN score is NaN.  Maxima pass over a NaN, sums do not: it is a sum of exactly zero that says "nothing seen"
+// (whatever was seen weighs at least 1 at its maximum).
 //
 // windowMmaKernel: the rows of all query heads that share a kv head are packed into one tile of BM = 16 WM rows
 // (row = query * G + head of the group), so that grouped heads read K and V once.  The keys that any row of the tile
@@ -400,11 +402,11 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
     float den = 0.0f;
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
-      const float mw = partM[w * WM + r / 16][r % 16];
-      if (mw == -INFINITY) continue; // this group saw nothing of the row
+      const float mw = partM[w * WM + r / 16][r % 16], lw = partL[w * WM + r / 16][r % 16];
+      if (lw == 0.0f) continue; // this group saw nothing of the row
       const float f = exp2f(mw - mx);
       const float4 x = *reinterpret_cast<const float4 *>(xo + (static_cast<size_t>(w) * BM + r) * D + d);
-      den += partL[w * WM + r / 16][r % 16] * f;
+      den += lw * f;
       acc.x = fmaf(x.x, f, acc.x);
       acc.y = fmaf(x.y, f, acc.y);
       acc.z = fmaf(x.z, f, acc.z);
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
         p.pl[part] = den;
       }
     } else {
-      const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+      const float inv = den == 0.0f ? 0.0f : 1.0f / den;
       uint2 w;
       w.x = wnPack<T>(acc.x * inv, acc.y * inv);
       w.y = wnPack<T>(acc.z * inv, acc.w * inv);
@@ -443,30 +445,32 @@ __global__ void __launch_bounds__(WN_THREADS, D <= 128 ? 2 : 1)
   for (int i = tid + split * WN_THREADS; i < BM * (D / 4); i += WN_THREADS * p.splits) {
     const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
     if (row >= liveRows) continue;
-    float ms[WN_CLUSTER], mx = -INFINITY, den = 0.0f;
+    float ms[WN_CLUSTER], ls[WN_CLUSTER], mx = -INFINITY, den = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int c = 0; c < WN_CLUSTER; ++c) {
       ms[c] = -INFINITY;
-      if (c < p.splits) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[c]) : "r"(remote(&rowM[r], c)));
+      ls[c] = 0.0f;
+      if (c < p.splits) {
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[c]) : "r"(remote(&rowM[r], c)));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ls[c]) : "r"(remote(&rowL[r], c)));
+      }
       mx = fmaxf(mx, ms[c]);
     }
 #pragma unroll
     for (int c = 0; c < WN_CLUSTER; ++c) {
-      if (ms[c] == -INFINITY) continue; // this part saw nothing of the row
+      if (ls[c] == 0.0f) continue; // this part saw nothing of the row
       const float f = exp2f(ms[c] - mx);
       float4 x;
-      float part;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote(&rowL[r], c)));
       asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                    : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(remote(xo + static_cast<size_t>(r) * D + d, c)));
-      den += part * f;
+      den += ls[c] * f;
       acc.x = fmaf(x.x, f, acc.x);
       acc.y = fmaf(x.y, f, acc.y);
       acc.z = fmaf(x.z, f, acc.z);
       acc.w = fmaf(x.w, f, acc.w);
     }
-    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
     uint2 w;
     w.x = wnPack<T>(acc.x * inv, acc.y * inv);
     w.y = wnPack<T>(acc.z * inv, acc.w * inv);
@@ -490,12 +494,12 @@ __global__ void __launch_bounds__(128) windowJoinKernel(T *__restrict__ out, Win
   float mx = -INFINITY;
   for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, pm[s]);
   float den = 0.0f;
-  for (int s = 0; s < p.splits; ++s) den += pm[s] == -INFINITY ? 0.0f : pl[s] * exp2f(pm[s] - mx);
-  const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+  for (int s = 0; s < p.splits; ++s) den += pl[s] == 0.0f ? 0.0f : pl[s] * exp2f(pm[s] - mx);
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   for (int d = lane * 4; d < D; d += 128) {
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s = 0; s < p.splits; ++s) {
-      if (pm[s] == -INFINITY) continue;
+      if (pl[s] == 0.0f) continue; // this part saw nothing of the row
       const float f = exp2f(pm[s] - mx);
       const float4 x = *reinterpret_cast<const float4 *>(po + static_cast<int64_t>(s) * D + d);
       acc.x = fmaf(x.x, f, acc.x);
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(128)
       }
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   T *orow = out + b * p.ob + head * p.oh + qi * p.os;
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {

@@ -64,7 +64,7 @@ __device__ __forceinline__ void awSoftmax(uint32_t (&sc)[4][32], uint32_t sAddr,
   const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
   float corr = 1.0f;
   if (ref == -INFINITY) {
-    ref = mx; // nothing was seen so far: O and l are zero
+    ref = mx; // nothing was seen so far: O and l are zero (or NaN)
   } else if ((mx - ref) * sl2 > 8.0f) {
     corr = fastExp2((ref - mx) * sl2);
     ref = mx;
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
       if (ok && tiles > 0 && !__all_sync(0xffffffffu, mbarWait(oFull + 8 * m, 0, abortP, 9))) ok = false;
       if (ok) {
         tcFenceAfter();
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T *orow = out + b * p.ob + (head0 + row % p.Gp) * p.oh + qi * p.os;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               uint4 v = make_uint4(0, 0, 0, 0); // a row that sees no key (O may never have been written)
-              if (l > 0.0f) {
+              if (l != 0.0f) { // a NaN among them
                 v.x = packPair<T>(__uint_as_float(r[g * 8]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
                 v.y = packPair<T>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
                 v.z = packPair<T>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
