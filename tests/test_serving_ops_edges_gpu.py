@@ -1,9 +1,16 @@
-"""Serving operators at their edges: NaN among the operands."""
+"""Serving operators at their edges: NaN among the operands, scales that the tensor-core kernels hand on, bad parents in a
+long cache, and calls whose first use is inside a recording."""
+
+import ctypes
+import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
-from serving import Kernels, window_seen
+from serving import Kernels, attend, check, tree_lines, window_seen
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -97,3 +104,109 @@ def test_nan_in_a_tree(kn, B, H, Hkv, D, N):
         k2[b, Hkv - 1, keys] = NAN
         poisoned[b, :, (Hkv - 1) * G:] = True
         check_poison(run(q, kd, k2), clean, poisoned)
+
+
+# ---- scales and parents in long caches -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [0.0, -0.5])
+@pytest.mark.parametrize("B,H,Hkv,D,room", [(1, 4, 1, 64, 4352), (5, 16, 8, 128, 4352), (18, 8, 8, 64, 4352), (2, 8, 2, 128, 300)])
+def test_tree_scales_that_are_not_positive(kn, scale, B, H, Hkv, D, room):
+    """The rows are planned for the tensor-core kernel (many parts, three, one) and computed by the other one."""
+    gen = torch.Generator().manual_seed(B)
+    T = 4
+    q, kd, vd = rand(gen, B, T, H, D), rand(gen, B, T, Hkv, D), rand(gen, B, T, Hkv, D)
+    k, v = rand(gen, B, Hkv, room, D), rand(gen, B, Hkv, room, D)
+    lens = torch.randint(0, room + 1, (B,), generator=gen).to(torch.int32)
+    lens[0] = room
+    parents = torch.tensor([[-1, 0, 0, 2]], dtype=torch.int32)
+    got = kn.tree(q, kd, vd, k, v, None, lens, parents, scale=scale)
+    related = tree_lines(parents[0].tolist())
+    for b in sorted({0, B // 2, B - 1}):
+        cached = (torch.arange(room) < lens[b]).expand(T, room)
+        keys, vals = torch.cat([k[b], kd[b].transpose(0, 1)], dim=1), torch.cat([v[b], vd[b].transpose(0, 1)], dim=1)
+        want, tol = attend(q[b].transpose(0, 1), keys, vals, torch.cat([cached, related], dim=1), scale, torch.bfloat16)
+        check(got[b].transpose(0, 1), want, tol, f"user {b}")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5])
+@pytest.mark.parametrize("N", [90, 700, 5000])
+def test_decode_scales_that_are_not_positive(kn, scale, N):
+    gen = torch.Generator().manual_seed(N)
+    q, k, v = rand(gen, 1, 1, 4, 64), rand(gen, 1, 2, N, 64), rand(gen, 1, 2, N, 64)
+    got = kn.decode(q, k, v, None, torch.tensor([N - 1], dtype=torch.int32), 10 ** 6, 0, scale=scale)
+    want, tol = attend(q[0, 0][:, None], k[0], v[0], torch.ones(1, N, dtype=torch.bool), scale, torch.bfloat16)
+    check(got[0, 0][:, None], want, tol)
+
+
+def test_tree_in_a_long_cache_reports_a_parent_that_is_not_an_earlier_node(kn):
+    gen = torch.Generator().manual_seed(2)
+    N = 4400
+    q, kd, vd = rand(gen, 1, 4, 4, 64), rand(gen, 1, 4, 2, 64), rand(gen, 1, 4, 2, 64)
+    k, v = rand(gen, 1, 2, N, 64), rand(gen, 1, 2, N, 64)
+    lens = torch.tensor([N - 7], dtype=torch.int32)
+    i32 = lambda *x: torch.tensor([x], dtype=torch.int32)
+    good = kn.tree(q, kd, vd, k, v, None, lens, i32(-1, 0, -1, 1))
+    assert kn.bad() == 0
+    for parent in (2, 3, 64, -5, 2 ** 31 - 1):
+        got = kn.tree(q, kd, vd, k, v, None, lens, i32(-1, 0, parent, 1))
+        assert kn.bad() == 1 and kn.bad() == 0
+        assert torch.equal(got, good)
+    # a node that does not exist may name any parent
+    got = kn.tree(q, kd, vd, k, v, None, lens, i32(-1, 0, 0, 77), draft_lens=torch.tensor([3], dtype=torch.int32))
+    assert kn.bad() == 0 and (got[0, 3] == 0).all()
+
+
+# ---- the first call of a process inside a recording --------------------------------------------------------------------
+FIRST = r"""
+import ctypes, math, sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from __graft_entry__ import load_package
+load_package()
+from ttmlir_b200 import runtime_api as rt
+from serving import Kernels, TAG
+kn = Kernels(rt)
+gen = torch.Generator().manual_seed(1)
+r = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16)
+i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+B, T, H, Hkv, D, n = 1, 4, 4, 2, 64, 5000
+q, kd, vd, k, v = r(B, T, H, D), r(B, T, Hkv, D), r(B, T, Hkv, D), r(B, Hkv, n, D), r(B, Hkv, n, D)
+q1, qp, kp, vp = r(1, 1, H, D), r(1, H, 130, D), r(1, Hkv, 130, D), r(1, Hkv, 130, D)
+logits, u = torch.randn(2, 9000, generator=gen), torch.tensor([0.3, 0.7])
+caches, pairs = [r(4, Hkv, 8, D)], i32([0, 2], [1, 3])
+up = kn.upload
+P = dict((name, up(t)) for name, t in dict(q=q, kd=kd, vd=vd, k=k, v=v, q1=q1, qp=qp, kp=kp, vp=vp, logits=logits, u=u, cache=caches[0], pairs=pairs,
+         lens=i32(4900), pos=i32(4800), parents=i32([-1, 0, 1, 0]), path=i32([0, 2, 3, 0]), count=i32(3), table=i32([1]), short=i32(2)).items())
+outs = dict(tree=kn.empty(q.shape, q.dtype), decode=kn.empty(q1.shape, q.dtype), prompt=kn.empty(qp.shape, q.dtype), token=kn.empty((2,), torch.int32))
+sizes = [kn.lib.ttb_sdpa_tree_workspace_bytes(*kn.args(B, T, H, Hkv, D, n)), kn.lib.ttb_sdpa_window_decode_workspace_bytes(*kn.args(1, H, Hkv, D, n, 10 ** 6, 0))]
+works = [kn.empty((max(s, 16),), torch.uint8) for s in sizes]
+arr, darr = (ctypes.c_void_p * 1)(P["cache"].value), (ctypes.c_void_p * 1)(P["kd"].value)
+stream, trace = ctypes.c_void_p(), ctypes.c_void_p()
+kn._check(kn.lib.ttb_stream_create(ctypes.byref(stream)))
+kn._check(kn.lib.ttb_trace_begin(stream))
+bf, sc = TAG[torch.bfloat16], 1 / math.sqrt(D)
+kn.call("ttb_paged_copy_blocks", arr, 1, P["pairs"], 2, bf, 4, Hkv, 8, D, stream)
+kn.call("ttb_paged_commit_draft", arr, darr, 1, P["table"], P["short"], P["path"], P["count"], bf, 1, T, Hkv, 4, 8, 1, D, stream)
+kn.call("ttb_sdpa_tree", P["q"], P["kd"], P["vd"], P["k"], P["v"], None, P["lens"], P["parents"], None, outs["tree"], bf, B, T, H, Hkv, 1, n, 1, D, 1, 0, 0, sc,
+        works[0], ctypes.c_size_t(sizes[0]), stream)
+kn.call("ttb_sdpa_window_decode", P["q1"], P["k"], P["v"], None, P["pos"], outs["decode"], bf, 1, H, Hkv, 1, n, 1, D, 10 ** 6, 0, sc, works[1],
+        ctypes.c_size_t(sizes[1]), stream)
+kn.call("ttb_sdpa_window", P["qp"], P["kp"], P["vp"], None, outs["prompt"], bf, 1, H, Hkv, 130, 130, D, None, None, None, None, 0, 40, 1, sc, stream)
+kn.call("ttb_sample_logits", P["logits"], P["u"], None, None, None, None, outs["token"], None, 0, 2, 9000, 9000, None, ctypes.c_size_t(0), stream)
+kn._check(kn.lib.ttb_trace_end(stream, ctypes.byref(trace)))
+kn._check(kn.lib.ttb_trace_launch(trace, stream))
+kn._check(kn.lib.ttb_stream_sync(stream))
+got = [kn.download(outs["tree"], q.shape, q.dtype), kn.download(outs["decode"], q1.shape, q.dtype), kn.download(outs["prompt"], qp.shape, q.dtype),
+       kn.download(outs["token"], (2,), torch.int32), kn.download(P["cache"], caches[0].shape, q.dtype)]
+want = [kn.tree(q, kd, vd, k, v, None, i32(4900), i32([-1, 0, 1, 0])), kn.decode(q1, k, v, None, i32(4800), 10 ** 6, 0), kn.window(qp, kp, vp, 0, 40, 1),
+        kn.sample(logits, u)[0], kn.commit(kn.copy_blocks(caches, pairs), [kd], i32([1]), i32(2), i32([0, 2, 3, 0]), i32(3))[0]]
+assert all(torch.equal(g, w) for g, w in zip(got, want)), [torch.equal(g, w) for g, w in zip(got, want)]
+assert kn.bad() == 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_record_into_a_trace(device):
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST.format(root=os.path.dirname(here), tests=here)
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip().endswith("same"), res.stdout + res.stderr
