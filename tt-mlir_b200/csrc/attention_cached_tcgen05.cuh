@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(AC_THREADS, 1)
     }
   }
 
+  drainAborted(abortP);
   tcFenceBefore();
   __syncthreads();
   if (warp == 12) {

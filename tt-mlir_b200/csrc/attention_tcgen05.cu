@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
   }
 
+  drainAborted(abortP);
   tcFenceBefore();
   __syncthreads();
   if (warp == 1) {
@@ -690,6 +691,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
   }
 
+  drainAborted(abortP);
   tcFenceBefore();
   __syncthreads();
   if (warp == 1) {

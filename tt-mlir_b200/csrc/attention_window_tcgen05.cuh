@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1)
     }
   }
 
+  drainAborted(abortP);
   tcFenceBefore();
   __syncthreads();
   if (warp == 1) {

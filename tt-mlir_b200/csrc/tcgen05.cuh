@@ -55,6 +55,15 @@ __device__ __forceinline__ bool mbarWait(uint32_t bar, uint32_t parity, volatile
   return true;
 }
 
+// Called by every thread behind its role and in front of the barrier that precedes the kernel's end.  After a wait that ran
+// out, copies and products of this CTA may still be in flight: whoever knows of it stays for about a millisecond, so that they
+// land before shared and tensor memory are released.
+__device__ __forceinline__ void drainAborted(volatile int *abortFlag) {
+  if (!*abortFlag) return;
+  const long long start = clock64();
+  while (clock64() - start < 2000000ll) __nanosleep(1000);
+}
+
 __device__ __forceinline__ void tmaLoad2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
