@@ -415,8 +415,8 @@ TTB_API int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draf
  *                           copied to many places; a pair of negatives is padding.  A destination must not be the source of
  *                           a pair nor the destination of another.  A pair that breaks this (of several with one
  *                           destination all but the first) or names a block outside the cache is left out and reported by
- *                           ttb_index_status.  Forks a sequence (its last, partly filled block), reorders beams, and moves
- *                           the live blocks behind a pool's new end into its holes.
+ *                           ttb_index_status.  A call takes at most 2^20 pairs.  Forks a sequence (its last, partly filled
+ *                           block), reorders beams, and moves the live blocks behind a pool's new end into its holes.
  *   ttb_paged_commit_draft  appends the accepted path of a draft tree: row path[b][i] of the draft [users, nodes, heads,
  *                           head_dim] becomes position cached_lens[b] + i of user b, for i < path_lens[b] (path Int32
  *                           [users, nodes], cached_lens and path_lens Int32 [users], page_table Int32 [users, pages]).  A row

@@ -155,6 +155,34 @@ def test_tree_in_a_long_cache_reports_a_parent_that_is_not_an_earlier_node(kn):
     assert kn.bad() == 0 and (got[0, 3] == 0).all()
 
 
+# ---- block copies -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("caches,blocks,moves", [(9, 2100, 1000), (5, 30, 12), (9, 50, 20), (260, 900, 420)])
+def test_copy_blocks_of_many_caches_and_pairs(kn, caches, blocks, moves):
+    """Each piece of a pair serves several caches in turn; among the pairs are paddings, blocks outside and destinations twice."""
+    gen = torch.Generator().manual_seed(blocks)
+    ts = [torch.randint(-128, 128, (blocks, 1, 2, 24), generator=gen, dtype=torch.int8) for _ in range(caches)]
+    order = torch.randperm(blocks, generator=gen).to(torch.int32)
+    pairs = torch.stack([order[:moves], order[blocks - moves:]], dim=1).contiguous()
+    assert kn.bad() == 0
+    done = torch.ones(moves, dtype=torch.bool)
+    pairs[3] = -1
+    done[3] = False
+    for g, t in zip(kn.copy_blocks(ts, pairs), ts):
+        want = t.clone()
+        want[pairs[done, 1].long()] = t[pairs[done, 0].long()]
+        assert torch.equal(g, want)
+    assert kn.bad() == 0
+    pairs[moves - 1, 1] = pairs[0, 1]       # a destination twice: the first stays
+    pairs[moves - 2, 0] = blocks            # outside
+    pairs[moves - 3, 1] = pairs[1, 0]       # onto a source
+    done[moves - 3:] = False
+    for g, t in zip(kn.copy_blocks(ts, pairs), ts):
+        want = t.clone()
+        want[pairs[done, 1].long()] = t[pairs[done, 0].long()]
+        assert torch.equal(g, want)
+    assert kn.bad() == 1
+
+
 # ---- the first call of a process inside a recording --------------------------------------------------------------------
 FIRST = r"""
 import ctypes, math, sys
