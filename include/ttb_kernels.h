@@ -470,8 +470,9 @@ TTB_API int ttb_sampling(const void *values, const void *indices, const void *k,
  *   uniform      in [0, 1): the token is the first index, in the vocabulary's order, at which the running sum of the weights
  *                that stayed exceeds uniform * their total
  * out (Int32 [rows]) gets the token and prob (f32 [rows], nullable) its share of the weights that stayed.  -inf and NaN
- * logits are never taken; a row of nothing else gives -1 and 0.  A weight below 2^-60 of the row's largest counts as
- * none.  vocab is limited to 2^22.  The same inputs give the same token on every run.
+ * logits are never taken; a row of nothing else gives -1 and 0.  A weight below 2^-60 of the row's largest may count as
+ * none.  Weights and their sums hold to 2^-36 of themselves: the token is the definition's unless uniform or top_p lies that
+ * near to a border.  vocab is limited to 2^22.  The same inputs give the same token on every run.
  * `workspace`: ttb_sample_logits_workspace_bytes(...), not shared by calls that can overlap on the GPU.
  * ttb_sampling draws among pre-selected candidates with its own generator (operations/reduction/sampling.cpp). */
 TTB_API size_t ttb_sample_logits_workspace_bytes(int64_t rows, int64_t vocab);

@@ -183,6 +183,109 @@ def test_copy_blocks_of_many_caches_and_pairs(kn, caches, blocks, moves):
     assert kn.bad() == 1
 
 
+# ---- sampling next to a border ---------------------------------------------------------------------------------------------
+def flat_rows(gen, rows, vocab, dtype, kind):
+    """Rows whose weight is spread over many tokens: noise under a few likely tokens, or one token over equal others."""
+    if kind == "noise":
+        x = torch.randn(rows, vocab, generator=gen) * 2.5
+        x.scatter_add_(1, torch.randint(0, vocab, (rows, 24), generator=gen), torch.rand(rows, 24, generator=gen) * 12)
+    else:
+        x = torch.full((rows, vocab), 0.7133)
+        x[torch.arange(rows), torch.randint(0, vocab, (rows,), generator=gen)] = 8 + 6 * torch.rand(rows, generator=gen)
+    return x.to(dtype)
+
+
+def near_border(shares, above):
+    """(i, u): a multiple u of 2^-24 in (0.5, 1), exact in f32, that lies 2^-31 .. 2^-29 above (below) shares[i]."""
+    steps = torch.ceil(shares * 2 ** 24) if above else torch.floor(shares * 2 ** 24)
+    far = (steps * 2.0 ** -24 - shares).abs()
+    ok = (far > 2.0 ** -31) & (far < 2.0 ** -29) & (shares > 0.5) & (shares < 0.999)
+    own = torch.diff(shares) > 2.0 ** -27                            # between neighbours that the distance does not reach
+    ok[1:-1] &= own[:-1] & own[1:]
+    ok[0] = ok[-1] = False
+    i = int(ok.nonzero()[0])
+    return i, float(steps[i] * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kind", ["noise", "equal"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_draws_next_to_a_border(kn, dtype, kind):
+    """u lies within 2^-29 of the border between two tokens.  The running sums' shares are off by less than 2^-36 (2^-38 for
+    each weight, above and below the fraction bar; f64 sums add 2^-36 of that), so the token is the definition's."""
+    gen = torch.Generator().manual_seed(71)
+    logits = flat_rows(gen, 24, 128000, dtype, kind)
+    us, want = [], []
+    for r in range(logits.shape[0]):
+        x = logits[r].double()
+        run = torch.cumsum(torch.exp(x - x.max()), 0)
+        i, u = near_border((run / run[-1])[1000:-1000], r % 2 == 0)
+        us.append(u)
+        want.append(1000 + i + (1 if r % 2 == 0 else 0))          # above the end of i's share: the next token
+    token, prob = kn.sample(logits, torch.tensor(us))
+    assert token.tolist() == want
+    x = logits.double()
+    w = torch.exp(x - x.amax(dim=1, keepdim=True))
+    share = w[torch.arange(len(want)), want] / w.sum(dim=1)
+    assert ((prob.double() - share).abs() <= 2.0 ** -23 * share).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [0, 60000])
+def test_sample_keeps_the_prefix_next_to_a_border(kn, dtype, k):
+    """top-p lies within 2^-29 of a prefix's share: one entry more or less would show in the share of the token drawn, which
+    is off by at most half a step of f32 and 2^-36."""
+    gen = torch.Generator().manual_seed(72)
+    logits = flat_rows(gen, 16, 128000, dtype, "noise")
+    ps, want, shares = [], [], []
+    u = torch.tensor(0.3)
+    for r in range(logits.shape[0]):
+        x = logits[r].double()
+        order = torch.sort(x, descending=True, stable=True).indices
+        kept = order[:k] if k else order
+        mass = torch.exp(x[kept] - x[order[0]])
+        run = torch.cumsum(mass, 0)
+        i, p = near_border((run / run[-1])[:40000], r % 2 == 0)
+        ps.append(p)
+        kept = kept[:i + (2 if r % 2 == 0 else 1)]                # above the prefix's share: it takes one more
+        kept = torch.sort(kept).values
+        mass = torch.exp(x[kept] - x[order[0]])
+        run = torch.cumsum(mass, 0)
+        at = int((run <= float(u) * run[-1]).sum())
+        want.append(int(kept[at]))
+        shares.append(float(mass[at] / run[-1]))
+    rows = logits.shape[0]
+    token, prob = kn.sample(logits, u.repeat(rows), None, torch.full((rows,), k, dtype=torch.int32), torch.tensor(ps))
+    assert token.tolist() == want
+    shares = torch.tensor(shares, dtype=torch.float64)
+    assert ((prob.double() - shares).abs() <= 2.0 ** -23 * shares).all()
+
+
+def test_sample_min_p_at_its_border(kn):
+    """min-p is the weight of one token, rounded down or up to f32: the token stays or goes.  Under a very high temperature
+    every finite logit weighs 1, which min-p 1 keeps."""
+    gen = torch.Generator().manual_seed(73)
+    x = torch.randn(12, 3000, generator=gen)
+    low, want = [], []
+    for r in range(12):
+        w = torch.exp(x[r].double() - x[r].double().max())
+        at = int(torch.sort(w, descending=True).indices[100 + r])
+        m = torch.tensor(float(w[at]), dtype=torch.float64).to(torch.float32)
+        inf = torch.tensor(float("inf") if r % 2 else 0.0)
+        m = torch.nextafter(m, inf) if (m.double() < w[at]) == bool(r % 2) else m
+        low.append(float(m))
+        want.append(int((w >= m.double()).sum()))
+        assert want[-1] == 100 + r + (0 if r % 2 else 1)
+    # a draw of u -> 1 takes the last token that stayed, in the vocabulary's order
+    token, _ = kn.sample(x, torch.full((12,), 1.0 - 2.0 ** -24), None, None, None, torch.tensor(low))
+    for r in range(12):
+        w = torch.exp(x[r].double() - x[r].double().max())
+        assert int(token[r]) == int((w >= low[r]).nonzero()[-1])
+    for heat in (float("inf"), 1e30):
+        u = torch.rand(12, generator=gen)
+        token, prob = kn.sample(x, u, torch.full((12,), heat), None, None, torch.ones(12))
+        assert token.tolist() == [min(int(float(v) * 3000), 2999) for v in u] and torch.allclose(prob, torch.tensor(1 / 3000))
+
+
 # ---- the first call of a process inside a recording --------------------------------------------------------------------
 FIRST = r"""
 import ctypes, math, sys

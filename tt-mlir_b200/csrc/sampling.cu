@@ -4,9 +4,9 @@
 //   top-p   of those, in the same order, the shortest prefix whose weight reaches p of their sum
 //   min-p   of those, the ones with w_i >= min_p
 //   draw    the first i, in index order, at which the running sum of what stayed exceeds u times its total
-// A weight below 2^-60 of the largest counts as none.  Weights are computed in f32 (relative error near 2^-21), sums
-// of up to 32 of them in f32, everything above in f64 in a fixed order, or as integers where atomics are involved: the
-// token does not depend on timing.
+// A weight below 2^-60 of the largest may count as none.  Weights are computed in f64 (relative error 2^-38) and summed in
+// f64 in a fixed order, or, where atomics are involved, as integers of 2^-36 of the largest among them: the token does not
+// depend on timing, and differs from the definition's only where u or p lies within some 2^-36 of a border.
 //
 // The work is to read the row; the floor is one pass over it at HBM speed.  One CTA per row (two rows per SM hide each
 // other's latencies), 16 warps, each streaming a run of consecutive indices:
@@ -19,11 +19,13 @@
 //    settings at once, unless top-k is deeper than that.
 //  * The draw is a search too: of the warps' runs the one that holds u times the total is split among the warps
 //    again, until there is a thread for each entry.  After a cut the last pass knows the runs' weights already.
-// Measured, 256 rows of 128000 f32 logits (131 MB, 20 us at HBM speed), us: no cut 45 (2.9 TB/s), largest logit 50, top-k
-// 50 69, top-k 40000 108, top-p 0.99 (flat rows) 167, everything mixed 141.  What bounds it: passes take 45 to 65 thousand
-// of a row's clocks each, with two rows per SM (their reads 38 at HBM speed; instruction issue and the exponentials are
-// close behind), the steps between them, which depend on one another and whose instructions are fetched for the first
-// time, 13 (sample), 6 to 12 (choosing an interval), 10 to 20 (border in the list) and 13 (draw).
+// Measured, 256 rows of 128000 f32 logits (131 MB, 20 us at HBM speed), us: largest logit 48, no cut 72, top-k 50 70, top-k
+// 50 and top-p 0.9 128, top-k 40000 180, top-p 0.99 (flat rows) 257, everything mixed 230.  With weights of f32 exponentials
+// it was 43, 41, 62, 79, 103, 166 and 141, and the tokens were not the definition's (see Weigher).  What bounds it: a pass
+// that weighs issues some 35 to 40 instructions per entry, 14 of them f64, and takes some 110 thousand of a row's clocks with
+// two rows per SM (one that only compares 50; their reads 38 at HBM speed); the steps between passes, which depend on one
+// another and whose instructions are fetched for the first time, 13 (sample), 6 to 12 (choosing an interval), 10 to 25
+// (border in the list) and 13 (draw).
 #include "common.cuh"
 
 #include <cfloat>
@@ -40,10 +42,13 @@ constexpr int SL_STAGES = 6;                // 16-byte vectors of a thread in fl
 constexpr int SL_BINS = 1024;               // two per thread
 constexpr float SL_FIRST = 2500.0f;         // entries aimed at by the first pass
 constexpr float SL_FLOOR = 60.0f;           // octaves below the largest weight that count
-constexpr float SL_UNIT = 68719476736.0f;   // 2^36 units to the largest weight: 2^13 of them fit two 32-bit halves
-constexpr int SL_HALF = 18;                 // ... of 18 bits each, whose sums stay below 2^31
+constexpr int SL_UNITS = 36;                // a list's largest weight is at most 2^36 units
+constexpr int SL_HALF = 18;                 // ... in two halves, which are summed as unsigned 32-bit numbers
+constexpr int SL_SIDE = 4;                  // weights computed side by side
+constexpr double SL_RISE = 900.0;           // octaves that a logit may lie above the reference
 constexpr int64_t SL_MAX_VOCAB = 1 << 22;
-static_assert(SL_BINS == 2 * SL_THREADS && SL_THREADS * SL_KEEP < 1 << 14, "bins per thread; the halves' sums fit 32 bits");
+static_assert(SL_BINS == 2 * SL_THREADS, "bins per thread");
+static_assert(int64_t(SL_THREADS) * SL_KEEP << SL_HALF < int64_t(1) << 32 && SL_UNITS == 2 * SL_HALF, "the halves' sums fit unsigned 32 bits");
 
 // What one pass found: entries and weight at and above lo and hi, the weight at and above a third bound and of everything,
 // the largest logit.
@@ -82,7 +87,7 @@ struct alignas(16) SampleSmem {
   float runTop[SL_WARPS];    // ... and the largest logit
   float border, lo, hi, high;
   unsigned int ties;
-  unsigned long long through;
+  double through;
 };
 
 template <typename V> __device__ __forceinline__ V slWarpSum(V v) {
@@ -110,30 +115,70 @@ template <typename V> __device__ __forceinline__ V slWarpScan(V v) {
   return v;
 }
 
-// Weights relative to a reference logit: 2^((x - ref) c).  Difference and product are each rounded once, so a weight 2^-h
-// is off by some h 2^-24 of itself.  Under an infinite temperature every finite logit weighs 1 (c = 0); the weight of
-// +-inf then has no value and is never asked for: entries of -inf fail the comparisons around it, and where the largest
-// logit is +inf only its count matters.
+// 2^f = 1 + f q(f) on [-1/2, 1/2], q interpolated in eight Chebyshev nodes: off by at most 2^-38 of itself.
+__constant__ double slExp2[8] = {0.69314718055683244,   0.24022650695888503,   0.055504109063258665, 0.0096181291352361396,
+                                 0.0013333478473685416, 0.00015403475186530786, 1.5303700711365693e-05, 1.325080551750225e-06};
+
+// Weights relative to a reference logit: 2^((x - ref) c) in f64 (weights of f32 exponentials gave some 8 in 10000 draws from
+// flat rows of 128000 another token than the definition's).  The exponent is split into the nearest integer n and f in
+// [-1/2, 1/2]; n goes into the exponent's bits.  Logits that weigh less than some 2^-400 are raised to there; above 2^1023
+// the bits overflow, so a sum is used only where the largest logit shows that none did (SL_RISE).  A NaN counts as the
+// smallest logit; -inf may weigh anything and is compared away.
 struct Weigher {
-  float ref, c;
+  double ref, c; // c: octaves per unit of a logit
+  float least;
   __device__ __forceinline__ void refer(float to, float heat) {
-    ref = heat < INFINITY ? to : 0.0f;
-    c = fminf(1.4426950408889634f / heat, 1e30f);
+    ref = to;
+    // Infinitely hot: every finite logit weighs 1.  Where one step of the logits' own grid is 100 octaves, more change nothing.
+    const double step = fmin(static_cast<double>(to) - static_cast<double>(nextafterf(to, -INFINITY)), 2.0282409603651670e31); // FLT_MAX's own: 2^104
+    c = fmin(fmax(1.4426950408889634 / static_cast<double>(heat), 1e-300), 100.0 / step);
+    least = fmaxf(static_cast<float>(ref - 400.0 / c), -FLT_MAX);
   }
-  __device__ __forceinline__ float operator()(float x) const {
-    float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((x - ref) * c));
+  // N weights side by side, so that a coefficient is fetched once for all of them.
+  template <int N> __device__ __forceinline__ void each(const float *x, double *w) const {
+    constexpr double MAGIC = 6755399441055744.0; // 1.5 * 2^52: the sum's low word is the nearest integer
+    double f[N];
+    unsigned int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double d = static_cast<double>(fmaxf(x[i], least)) - ref, m = fma(d, c, MAGIC);
+      f[i] = fma(d, c, MAGIC - m);
+      n[i] = static_cast<unsigned int>(__double2loint(m)) << 20;
+      w[i] = slExp2[7];
+    }
+#pragma unroll
+    for (int k = 6; k >= -1; --k) {
+      const double a = k < 0 ? 1.0 : slExp2[k < 0 ? 0 : k];
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = fma(f[i], w[i], a);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __hiloint2double(__double2hiint(w[i]) + static_cast<int>(n[i]), __double2loint(w[i]));
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    double w;
+    each<1>(&x, &w);
     return w;
+  }
+  __device__ __forceinline__ float octaves() const { return fminf(static_cast<float>(c), 1e30f); }
+  // The smallest logit whose weight is at least w (0 < w <= 1).
+  __device__ __forceinline__ float reaches(double w) const {
+    float x = static_cast<float>(ref + (log2(w) - 1.6e-16) / c); // within a step or two (a weight within 2^-53 of 1 is 1)
+    if (!(x > -FLT_MAX)) return -FLT_MAX;
+    for (int i = 0; i < 4; ++i) x = nextafterf(x, -INFINITY);
+    for (int i = 0; i < 8 && (*this)(x) < w; ++i) x = nextafterf(x, INFINITY);
+    return x;
   }
 };
 
-// Calls f(v) for entries lo .. hi - 1 of a row, a few of them (an array) per lane at a time, all 32 lanes together; an
+// Calls f(v) for entries lo .. hi - 1 of a row, N (4 or 8) of them (an array) per lane at a time, all 32 lanes together; an
 // entry that a lane does not have is -inf.  f lets the warp vote on all of them.  The 16-byte vectors of a range are cut
 // into steps of 256 entries; the ragged ends come last.  Vectors come through a ring in shared memory that each lane
 // fills and reads for itself, which keeps them in flight without registers.
-template <typename T, typename F>
+template <int N, typename T, typename F>
 __device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, int hi, F &&f) {
   constexpr int VEC = 16 / sizeof(T), PER = 8 / VEC, AHEAD = SL_STAGES / PER; // entries per vector, vectors per step, steps in flight
+  constexpr int TAKE = N < VEC ? N : VEC;
   const int lane = threadIdx.x & 31;
   if (lo >= hi) return;
   const int skip = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / static_cast<int>(sizeof(T));
@@ -157,16 +202,21 @@ __device__ __forceinline__ void slForRange(const T *x, SampleSmem *s, int lo, in
 #pragma unroll 1
   for (int c = 0; c < steps; ++c) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(AHEAD - 1) : "memory");
-    float v[8];
+#pragma unroll 2
+    for (int u = 0; u < 8; u += N) { // fours are fetched from the ring one after the other: fewer registers
+      float v[N];
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const uint4 raw = ring[(stage * PER + u) * SL_THREADS];
-      const T *e = reinterpret_cast<const T *>(&raw);
+      for (int i0 = 0; i0 < N; i0 += TAKE) {
+        struct alignas(TAKE * sizeof(T)) Piece {
+          T e[TAKE];
+        };
+        const Piece raw = *reinterpret_cast<const Piece *>(reinterpret_cast<const T *>(ring + (stage * PER + (u + i0) / VEC) * SL_THREADS) + (u + i0) % VEC);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[u * VEC + i] = toF32(e[i]);
+        for (int i = 0; i < TAKE; ++i) v[i0 + i] = toF32(raw.e[i]);
+      }
+      f(v);
     }
-    f(v);
-    fetch(c + AHEAD, stage); // f has voted on every entry: they have arrived, the stage is free
+    fetch(c + AHEAD, stage); // this lane has read its column of the stage: it is free
     stage = stage + 1 < AHEAD ? stage + 1 : 0;
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
@@ -211,14 +261,14 @@ __device__ __forceinline__ float slMax3(float a, float b, float c) { // a NaN co
 // hi is +inf; otherwise FIRST also weighs what lies at and above `high`.  A step first asks whether any of the lanes'
 // entries can lie in the interval, and mostly none does.
 template <bool FIRST, bool OPEN, bool WEIGHTS, typename T>
-__device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s, const Weigher &weigh, float lo, float hi, float high) {
+__device__ __forceinline__ unsigned int slPass(const T *row, int n, SampleSmem *s, const Weigher &weigh, float lo, float hi, float high) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float top = -INFINITY, fLo = 0.0f, fHi = 0.0f, fHigh = 0.0f, fAll = 0.0f, farCount = 0.0f; // farCount stays below 2^24
+  float top = -INFINITY, farCount = 0.0f; // farCount stays below 2^24
   double mLo = 0.0, mHi = 0.0, mHigh = 0.0, mAll = 0.0;
-  unsigned int mine = 0, steps = 0;
+  unsigned int mine = 0;
   const float middle = FIRST ? 0.0f : 0.5f * lo + 0.5f * hi, reach = FIRST ? 0.0f : fmaxf(hi - middle, middle - lo) * 1.000001f;
   float *column = &s->list[0][threadIdx.x];
-  slForRange(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
+  slForRange<WEIGHTS ? 4 : 8>(row, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
     constexpr int N = sizeof(v) / sizeof(float);
     bool near;
     if (FIRST) {
@@ -232,41 +282,44 @@ __device__ __forceinline__ unsigned int slPass(const T *x, int n, SampleSmem *s,
 #pragma unroll
       for (int i = 0; i < N; ++i) m = fminf(m, fabsf(v[i] - middle));
       near = !(m > reach);
-    }
+      float most = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float w = WEIGHTS ? weigh(v[i]) : 0.0f;
-      if (WEIGHTS && FIRST && v[i] > -INFINITY) fAll += w;
-      if (!OPEN && v[i] >= hi) {
-        farCount += 1.0f;
-        if (WEIGHTS) fHi += w;
+      for (int i = 0; i < N; i += 2) most = slMax3(most, v[i], v[i + 1]);
+      if (!__any_sync(0xffffffffu, near || most >= hi)) return; // nothing of interest to anyone
+    }
+    const bool collect = __any_sync(0xffffffffu, near);
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += SL_SIDE) {
+      double w[SL_SIDE];
+      if (WEIGHTS) weigh.template each<SL_SIDE>(v + i0, w);
+#pragma unroll
+      for (int k = 0; k < SL_SIDE; ++k) {
+        const float x = v[i0 + k];
+        if (WEIGHTS && FIRST && x > -INFINITY) mAll += w[k];
+        if (!OPEN && x >= hi) {
+          farCount += 1.0f;
+          if (WEIGHTS) mHi += w[k];
+        }
+        if (FIRST && !OPEN && WEIGHTS && x >= high) mHigh += w[k];
       }
-      if (FIRST && !OPEN && WEIGHTS && v[i] >= high) fHigh += w;
-    }
-    if (__any_sync(0xffffffffu, near)) {
+      if (!collect) continue;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (v[i] >= lo && v[i] < hi) {
-          if (mine < SL_KEEP) column[mine * SL_THREADS] = v[i];
+      for (int k = 0; k < SL_SIDE; ++k) {
+        const float x = v[i0 + k];
+        if (x >= lo && x < hi) {
+          if (mine < SL_KEEP) column[mine * SL_THREADS] = x;
           ++mine;
-          if (WEIGHTS) fLo += weigh(v[i]);
+          if (WEIGHTS) mLo += w[k];
         }
       }
-    }
-    if (WEIGHTS && (++steps & 3) == 0) { // a few f32 sums at a time
-      mLo += fLo;
-      mHi += fHi;
-      mHigh += fHigh;
-      mAll += fAll;
-      fLo = fHi = fHigh = fAll = 0.0f;
     }
   });
   unsigned int cHi = static_cast<unsigned int>(farCount);
   if (WEIGHTS) {
-    mHi = OPEN ? 0.0 : slWarpSum(mHi + fHi);
-    mLo = slWarpSum(mLo + fLo) + mHi; // at and above lo
-    if (FIRST) mAll = slWarpSum(mAll + fAll);
-    if (FIRST && !OPEN) mHigh = slWarpSum(mHigh + fHigh);
+    mHi = OPEN ? 0.0 : slWarpSum(mHi);
+    mLo = slWarpSum(mLo) + mHi; // at and above lo
+    if (FIRST) mAll = slWarpSum(mAll);
+    if (FIRST && !OPEN) mHigh = slWarpSum(mHigh);
   }
   top = slWarpMax(top);
   cHi = slWarpSum(cHi);
@@ -332,14 +385,31 @@ __device__ __forceinline__ void slSpan(SampleSmem *s, float &a, float &b) {
   __syncthreads();
 }
 
-// The border among the collected entries, which lie in [least, most] (this thread holds `count`): the first `rest` in
-// descending order, or (byMass) entries as long as the units in front of them are fewer than `rest`.  Leaves s->border,
-// s->ties and (weights) s->through, the units of the entries that stay.
-__device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, unsigned int count, bool byMass, bool weights, unsigned long long rest,
-                                         float least, float most) {
+// The border among the collected entries, which lie in [least, most] (this thread holds `count`): the first `limit` in
+// descending order, or (byMass) entries as long as the weight in front of them is below `limit`.  Leaves s->border, s->ties
+// and (weights) s->through, the weight of the entries that stay.  Weights are taken in units of a power of two that suits the
+// largest possible one.
+__device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, unsigned int count, bool byMass, bool weights, double limit, float least,
+                                         float most) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float *column = &s->list[0][threadIdx.x];
-  auto units = [&](float v) { return __float2ull_rn(weigh(v) * SL_UNIT); };
+  const int shift = min(SL_UNITS - 1 + 1023 - (__double2hiint(weigh(most)) >> 20), 1000); // weigh(most) < 2^SL_UNITS units
+  const double unit = __hiloint2double((1023 + shift) << 20, 0);
+  auto units = [&](double w) { return __double2ull_rn(w * unit); };
+  // f(value, weight) for this thread's entries, SL_SIDE side by side; a value past the last is NaN.
+  auto forList = [&](bool weighed, auto &&f) {
+#pragma unroll 1
+    for (unsigned int i = 0; i < count; i += SL_SIDE) {
+      float v[SL_SIDE];
+      double w[SL_SIDE];
+#pragma unroll
+      for (int k = 0; k < SL_SIDE; ++k) v[k] = i + k < count ? column[(i + k) * SL_THREADS] : NAN;
+      if (weighed) weigh.template each<SL_SIDE>(v, w);
+#pragma unroll
+      for (int k = 0; k < SL_SIDE; ++k) f(v[k], weighed ? w[k] : 0.0);
+    }
+  };
+  unsigned long long rest = static_cast<unsigned long long>(fmax(byMass ? ceil(limit * unit) : limit, 1.0));
   for (bool settled = false; !settled;) {
 #pragma unroll 1
     for (int i = threadIdx.x; i < SL_BINS; i += SL_THREADS) s->count[i] = s->massLo[i] = s->massHi[i] = 0;
@@ -348,19 +418,17 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
     // A range that overflows is shrunk first; one so narrow that the step overflows still separates its ends.
     const float shrink = most - least < INFINITY ? 1.0f : 0.25f, base = least * shrink, step = (SL_BINS - 1) / (most * shrink - base);
     auto binOf = [&](float v) { return max(0, min(static_cast<int>(fmaf(v, shrink, -base) * step), SL_BINS - 1)); }; // rounded alike in both uses
-#pragma unroll 4
-    for (unsigned int i = 0; i < count; ++i) {
-      const float v = column[i * SL_THREADS];
+    forList(byMass, [&](float v, double w) {
       if (v >= least && v <= most) {
         const int bin = binOf(v);
         atomicAdd(&s->count[bin], 1u);
         if (byMass) {
-          const unsigned long long w = units(v);
-          atomicAdd(&s->massLo[bin], static_cast<unsigned int>(w & ((1u << SL_HALF) - 1u)));
-          atomicAdd(&s->massHi[bin], static_cast<unsigned int>(w >> SL_HALF));
+          const unsigned long long u = units(w);
+          atomicAdd(&s->massLo[bin], static_cast<unsigned int>(u & ((1u << SL_HALF) - 1u)));
+          atomicAdd(&s->massHi[bin], static_cast<unsigned int>(u >> SL_HALF));
         }
       }
-    }
+    });
     __syncthreads();
     // descending bins: thread t holds bins SL_BINS - 1 - 2t and the one below
     const int b0 = SL_BINS - 1 - 2 * static_cast<int>(threadIdx.x), b1 = b0 - 1;
@@ -397,7 +465,7 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
       if (warp == 0) {
         const bool live = lane < inBin;
         const float v = live ? s->few[lane] : -INFINITY;
-        const unsigned long long each = byMass ? units(v) : 1ull;
+        const unsigned long long each = byMass ? units(weigh(v)) : 1ull;
         unsigned long long inFront = 0;
         unsigned int equal = 0;
 #pragma unroll 1
@@ -437,17 +505,13 @@ __device__ __forceinline__ void slSelect(SampleSmem *s, const Weigher &weigh, un
     __syncthreads();
   }
   const float border = s->border;
-  const unsigned long long each = units(border), per = byMass ? each : 1ull, equal = s->equal;
+  const unsigned long long each = units(weigh(border)), per = byMass ? each : 1ull, equal = s->equal;
   unsigned long long keep = per ? (s->rest + per - 1) / per : equal, above = 0, through;
   keep = keep < 1 ? 1 : (keep > equal ? equal : keep); // a rounded limit may ask for more than there are
   if (weights) {
-#pragma unroll 4
-    for (unsigned int i = 0; i < count; ++i) {
-      const float v = column[i * SL_THREADS];
-      above += v > border ? units(v) : 0ull;
-    }
+    forList(true, [&](float v, double w) { above += v > border ? units(w) : 0ull; });
     slScan<unsigned long long>(above, s->uRed[0], through);
-    if (threadIdx.x == 0) s->through = through + keep * each;
+    if (threadIdx.x == 0) s->through = static_cast<double>(through + keep * each) * __hiloint2double((1023 - shift) << 20, 0);
   }
   if (threadIdx.x == 0) s->ties = static_cast<unsigned int>(keep);
   __syncthreads();
@@ -558,65 +622,83 @@ __device__ __forceinline__ void slChoose(SampleSmem *s, float c, float below, fl
   }
 }
 
-// The draw among the entries above `border` and the first `ties` equal to it, with a weight of at least `low`.  The row is
+// The draw among the entries above `border` and the first `ties` equal to it, none of them below `low`.  The row is
 // weighed by the 16 runs of slPass, the run that holds u times the total by 16 runs again, until there is a thread for
 // each entry that is left.  The last pass may have left what is needed of the runs: KNOWN_LIST, this thread's `count` entries (all that
 // stay below hi) and s->runAbove (times `scale`); KNOWN_TOP, s->runTop (the first of the largest logits is drawn).
-// False: the total is out of range.
+// False: a logit lies too far above the reference.
 template <typename T>
-__device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const Weigher &weigh, float border, unsigned int ties, float low, double u, int known,
-                                       unsigned int count, double scale, int32_t *out, float *prob) {
+__device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const Weigher &weigh, float border, unsigned int ties, float low, double u, bool exactTop,
+                                       int known, unsigned int count, double scale, int32_t *out, float *prob) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float wBorder = border < INFINITY ? (border > -INFINITY ? weigh(border) : 0.0f) : 1.0f;
-  const double wEqual = wBorder >= low ? static_cast<double>(wBorder) : 0.0;
-  float f = 0.0f;
-  auto weighUp = [&](float v) {
-    const float w = weigh(v);
-    if (v > border && !(w < low)) f += w; // an overflowed weight (inf, or NaN) must show in the total
-    return v == border;
+  // counts: above the border, and no lighter than `low` (border +inf: nothing does, a NaN compares false)
+  const float above = border < INFINITY ? fmaxf(nextafterf(border, INFINITY), low) : NAN;
+  const double wEqual = border >= low ? (border < INFINITY ? weigh(border) : 1.0) : 0.0;
+  double sum = 0.0;
+  auto weighUp = [&](const auto &v) { // a few entries
+    constexpr int N = sizeof(v) / sizeof(float), SIDE = N < SL_SIDE ? N : SL_SIDE;
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += SIDE) {
+      bool some = false; // mostly none, when the border is high
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) some |= v[i0 + k] >= above;
+      if (!some) continue;
+      double w[SIDE];
+      weigh.template each<SIDE>(v + i0, w);
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) {
+        if (v[i0 + k] >= above) sum += w[k];
+      }
+    }
   };
   int from = 0, to = n;
   for (bool whole = true; whole || to - from > SL_THREADS; whole = false) {
     const int part = (to - from + SL_WARPS - 1) / SL_WARPS;
-    double sum = 0.0;
-    unsigned int equal = 0, steps = 0;
-    f = 0.0f;
+    unsigned int equal = 0;
+    float big = -INFINITY; // largest logit, while it is not known
+    sum = 0.0;
     if (!whole) {
       const int lo = min(to, from + warp * part), hi = min(to, lo + part);
 #pragma unroll 1
       for (int i0 = lo + lane; i0 < hi; i0 += 32 * 16) {
         float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = i0 + 32 * i < hi ? fmaxf(toF32(x[i0 + 32 * i]), -INFINITY) : -INFINITY;
+        for (int i = 0; i < 16; ++i) v[i] = i0 + 32 * i < hi ? toF32(x[i0 + 32 * i]) : NAN;
+        weighUp(v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) equal += weighUp(v[i]) && i0 + 32 * i < hi;
-        sum += f;
-        f = 0.0f;
+        for (int i = 0; i < 16; ++i) equal += v[i] == border;
       }
     } else if (known == KNOWN_LIST) { // at most SL_KEEP of them
-#pragma unroll 4
-      for (unsigned int i = 0; i < count; ++i) equal += weighUp(s->list[i][threadIdx.x]);
+#pragma unroll 1
+      for (unsigned int i = 0; i < count; i += SL_SIDE) {
+        float v[SL_SIDE];
+#pragma unroll
+        for (int k = 0; k < SL_SIDE; ++k) v[k] = i + k < count ? s->list[i + k][threadIdx.x] : NAN;
+        weighUp(v);
+#pragma unroll
+        for (int k = 0; k < SL_SIDE; ++k) equal += v[k] == border;
+      }
     } else if (known == KNOWN_TOP) {
       equal = lane == 0 && s->runTop[warp] == border;
     } else {
-      slForRange(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
+      slForRange<4>(x, s, slRun(n, warp), slRun(n, warp + 1), [&](auto &v) {
         constexpr int N = sizeof(v) / sizeof(float);
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < N; ++i) any |= weighUp(v[i]);
-        if (__any_sync(0xffffffffu, any)) {
+        weighUp(v);
+        if (ties) {
 #pragma unroll
           for (int i = 0; i < N; ++i) equal += v[i] == border;
         }
-        if ((++steps & 3) == 0) {
-          sum += f;
-          f = 0.0f;
+        if (!exactTop) {
+#pragma unroll
+          for (int i = 0; i < N; i += 2) big = slMax3(big, v[i], v[i + 1]);
         }
       });
+      if (!exactTop) big = slWarpMax(big);
     }
-    sum = slWarpSum(sum + f);
+    sum = slWarpSum(sum);
     equal = slWarpSum(equal);
     if (lane == 0) {
+      s->fRed[0][warp] = big;
       s->dRed[0][warp] = whole && known == KNOWN_LIST ? sum + s->runAbove[warp] * scale : sum;
       s->cRed[0][warp] = equal;
     }
@@ -629,6 +711,7 @@ __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const W
       const double run = slWarpScan(m);
       const double total = __shfl_sync(0xffffffffu, run, 31), target = whole ? u * total : s->target;
       const unsigned int hit = __ballot_sync(0xffffffffu, m > 0.0 && run > target), any = __ballot_sync(0xffffffffu, m > 0.0);
+      const float largest = slWarpMax(mine ? s->fRed[0][lane] : -INFINITY);
       // none: u = 1, or the last bit of a sum taken in another order: the last run that weighs anything
       const int at = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : SL_WARPS - 1);
       if (lane == at) {
@@ -639,7 +722,7 @@ __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const W
         s->to = whole ? slRun(n, lane + 1) : min(to, lo + part);
         if (whole) {
           s->total = total;
-          s->ok = total > 0.0 && total < 1e300;
+          s->ok = exactTop || (static_cast<double>(largest) - weigh.ref) * weigh.c < SL_RISE;
         }
       }
     }
@@ -655,13 +738,14 @@ __device__ __forceinline__ bool slPick(const T *x, int n, SampleSmem *s, const W
     s->pickBin[1] = -1;
   }
   const int i = from + static_cast<int>(threadIdx.x);
-  const float v = i < to ? fmaxf(toF32(x[i]), -INFINITY) : -INFINITY;
-  f = 0.0f;
-  const bool same = weighUp(v) && i < to;
+  const float v[1] = {i < to ? toF32(x[i]) : NAN};
+  sum = 0.0;
+  weighUp(v);
+  const bool same = v[0] == border;
   unsigned int allSame;
   double all;
   const unsigned int rank = s->equalBefore + slScan<unsigned int>(same, s->cRed[0], allSame);
-  const double mine = same ? (rank < ties ? wEqual : 0.0) : static_cast<double>(f), before = slScan<double>(mine, s->dRed[0], all);
+  const double mine = same ? (rank < ties ? wEqual : 0.0) : sum, before = slScan<double>(mine, s->dRed[0], all);
   if (mine > 0.0) {
     if (before + mine > s->target) atomicMin(&s->pickBin[0], static_cast<int>(threadIdx.x));
     atomicMax(&s->pickBin[1], static_cast<int>(threadIdx.x));
@@ -696,7 +780,7 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
   const int32_t k = topK ? topK[row] : 0;
   const float p = topP ? topP[row] : 1.0f;
   const bool cutK = !greedy && k > 0 && k < n, cutP = !greedy && p > 0.0f && p < 1.0f;
-  const float low = !greedy && minP && minP[row] > 0.0f && minP[row] <= 1.0f ? minP[row] : 0.0f;
+  const float share = !greedy && minP && minP[row] > 0.0f && minP[row] <= 1.0f ? minP[row] : 0.0f;
   const double u = fmin(fmax(static_cast<double>(uniform[row]), 0.0), 1.0); // NaN: 0
 
   // ---- a sample: evenly spaced, or all of a short row
@@ -735,17 +819,18 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
   const bool cut = cutK || cutP;
   // Without cuts and a min-p the draw needs no search: weights relative to the sample's largest logit will do, unless
   // that is so small that they overflow.
-  bool exactTop = false, search = cut || greedy || low > 0.0f || !(sTop > -INFINITY && sTop < INFINITY);
+  bool exactTop = false, search = cut || greedy || share > 0.0f || !(sTop > -INFINITY && sTop < INFINITY);
   weigh.refer(sTop, greedy ? 1.0f : heat);
   for (;;) {
     int known = KNOWN_NOTHING;
     unsigned int listed = 0; // entries this thread collected in the last pass
     double scale = 1.0;      // of that pass's weights to the present reference
+    float listEnd = INFINITY;
     if (search) {
       // The list holds the entries in [lo, hi); the border of the cut at work lies in [below, above).
       bool first = true, again = false, byMass = false, infinite = false, up = false;
       bool ask = cut && n > SL_SHORT && sTop > -INFINITY && sTop < INFINITY; // choose an interval first
-      float below = fmaxf(fmaxf(sTop - SL_FLOOR / weigh.c, -FLT_MAX), sLeast), above = INFINITY, floor = below, top = sTop;
+      float below = fmaxf(fmaxf(sTop - SL_FLOOR / weigh.octaves(), -FLT_MAX), sLeast), above = INFINITY, floor = below, top = sTop;
       float lo = cut ? -FLT_MAX : INFINITY, hi = INFINITY, want = static_cast<float>(k), have = 0.0f, borderK = -INFINITY;
       float firstLo = INFINITY, firstHi = INFINITY, high = INFINITY; // where the first pass knows the weight above
       unsigned int tiesK = 0xffffffffu;
@@ -754,8 +839,8 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
       int which = cutK ? 0 : 1, round = 0;
       for (bool done = false; !done;) {
         if (ask) {
-          // The first interval is open unless top-k is too deep for that (top-k 40000: 154 us with an open one, 108 closed).
-          slChoose(s, weigh.c, below, above, sLeast, top, byMass, first ? !cutK || want <= 0.6f * SL_FIRST : up, want, have, n, samples);
+          // The first interval is open unless top-k is too deep for that (top-k 40000: 154 us with an open one, 108 closed, with weights in f32).
+          slChoose(s, weigh.octaves(), below, above, sLeast, top, byMass, first ? !cutK || want <= 0.6f * SL_FIRST : up, want, have, n, samples);
           float nLo = s->lo, nHi = s->hi;
           if (first) {
             nLo = fminf(nLo, sTop);
@@ -800,6 +885,7 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           }
           exactTop = true;
           const double rise = (static_cast<double>(cur.top) - static_cast<double>(sTop)) * weigh.c;
+          const double unit = weigh.c;
           weigh.refer(cur.top, greedy ? 1.0f : heat);
           if (greedy) {
             border = cur.top;
@@ -817,16 +903,16 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           // From here on weights are relative to the true largest logit; the first pass's are rescaled, or taken again
           // when its reference was so far off that they may have overflowed (or there was none).
           if (!again && (cutP || hi < INFINITY)) {
-            if (!(rise < 60.0)) {
+            if (!(rise < SL_RISE) || weigh.c != unit) {
               again = true;
               ask = false;
               continue;
             }
-            scale = static_cast<double>(exp2f(static_cast<float>(-rise)));
+            scale = weigh(sTop);
           }
           first = false;
           top = cur.top;
-          floor = fmaxf(top - SL_FLOOR / weigh.c, -FLT_MAX);
+          floor = fmaxf(top - SL_FLOOR / weigh.octaves(), -FLT_MAX);
           total = cur.mAll * scale;
           mHi = cur.mHi * scale;
           mLo = cur.mLo * scale;
@@ -856,12 +942,11 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
           up = false;
           if (limit > hiAt && limit <= loAt) {
             if (cur.fits) {
-              const double rest = byMass ? ceil((limit - hiAt) * static_cast<double>(SL_UNIT)) : limit - hiAt;
-              slSelect(s, weigh, listed, byMass, cutP, static_cast<unsigned long long>(fmax(rest, 1.0)), lo, fminf(hi, top));
+              slSelect(s, weigh, listed, byMass, cutP, limit - hiAt, lo, fminf(hi, top));
               border = s->border;
               ties = s->ties;
               known = KNOWN_LIST;
-              total = mHi + static_cast<double>(s->through) / static_cast<double>(SL_UNIT);
+              total = mHi + s->through;
               found = true;
             } else {
               if (lo > below) {
@@ -874,7 +959,7 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
               }
               if (above <= nextafterf(below, INFINITY)) { // one value, more often than the list is long
                 border = below;
-                const double w = static_cast<double>(weigh(below)), each = byMass ? fmax(w, 1e-300) : 1.0;
+                const double w = weigh(below), each = byMass ? fmax(w, 1e-300) : 1.0;
                 const double keep = fmin(fmax(ceil((limit - hiAt) / each), 1.0), static_cast<double>(cur.cLo - cur.cHi));
                 ties = static_cast<unsigned int>(keep);
                 total = mHi + keep * w;
@@ -948,10 +1033,11 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
         ties = 0xffffffffu;
         known = KNOWN_NOTHING;
       }
-      // What lies above the list must stay as a whole: a min-p that may reach into it asks for another look.
-      if (known == KNOWN_LIST && hi < INFINITY && !(weigh(hi) > 1.0001f * low)) known = KNOWN_NOTHING;
+      listEnd = hi;
     }
-    if (slPick(x, n, s, weigh, border, ties, low, u, known, listed, scale, out, prob) || exactTop) return;
+    const float low = share > 0.0f ? weigh.reaches(share) : fmaxf(static_cast<float>(weigh.ref - static_cast<double>(SL_FLOOR) / weigh.c), -FLT_MAX);
+    if (known == KNOWN_LIST && listEnd < low) known = KNOWN_NOTHING; // what lies above the list must stay as a whole
+    if (slPick(x, n, s, weigh, border, ties, low, u, exactTop, known, listed, scale, out, prob) || exactTop) return;
     search = true; // nothing was cut, and the sample's largest logit was too small a reference
     __syncthreads();
   }
