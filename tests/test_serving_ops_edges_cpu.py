@@ -2,7 +2,7 @@
 
 import pytest
 
-from test_serving_ops_cpu import COPY, INVALID, call, with_args
+from test_serving_ops_cpu import COPY, INVALID, N, WINDOW, call, with_args
 
 
 @pytest.mark.parametrize("pairs", [(1 << 20) + 1, (1 << 31) - 1])
@@ -10,3 +10,15 @@ def test_copy_blocks_refuses_more_pairs_than_a_launch_can_check(rt, pairs):
     """Each pair is checked against all others: without a limit a call could keep the GPU busy for minutes."""
     rc, text = call(rt, "ttb_paged_copy_blocks", with_args(COPY, np=pairs, heads=1, bs=1, d=8))
     assert rc == INVALID and "2^20" in text, (rc, text)
+
+
+@pytest.mark.parametrize("nulls", [("q", "out"), ("q", "k", "v", "out")])
+def test_a_prompt_without_queries_needs_no_addresses(rt, nulls):
+    rc, text = call(rt, "ttb_sdpa_window", with_args(WINDOW, sq=0, **{n: N for n in nulls}))
+    assert rc == 0, text
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "out"])
+def test_a_prompt_with_queries_and_keys_needs_addresses(rt, name):
+    rc, text = call(rt, "ttb_sdpa_window", with_args(WINDOW, **{name: N}))
+    assert rc == INVALID and "null" in text

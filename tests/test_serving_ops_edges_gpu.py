@@ -10,7 +10,7 @@ import sys
 import pytest
 import torch
 
-from serving import Kernels, attend, check, tree_lines, window_seen
+from serving import TAG, Kernels, attend, check, tree_lines, window_seen
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -104,6 +104,14 @@ def test_nan_in_a_tree(kn, B, H, Hkv, D, N):
         k2[b, Hkv - 1, keys] = NAN
         poisoned[b, :, (Hkv - 1) * G:] = True
         check_poison(run(q, kd, k2), clean, poisoned)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 256), (torch.float32, 64)])
+def test_a_prompt_without_keys_is_zero(kn, dtype, D):
+    q = rand(torch.Generator().manual_seed(1), 2, 4, 40, D, dtype=dtype)
+    out = kn.upload(torch.ones_like(q))
+    kn.call("ttb_sdpa_window", kn.up(q), None, None, None, out, TAG[dtype], 2, 4, 2, 40, 0, D, None, None, None, None, 0, 8, 1, 0.1, kn.stream)
+    assert (kn.download(out, q.shape, dtype) == 0).all()
 
 
 # ---- scales and parents in long caches -----------------------------------------------------------------------------------

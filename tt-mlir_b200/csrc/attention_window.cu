@@ -765,7 +765,7 @@ int ttb_sdpa_window(const void *q, const void *k, const void *v, const void *kv_
                     int64_t heads_kv, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int64_t *q_strides3, const int64_t *k_strides3,
                     const int64_t *v_strides3, const int64_t *out_strides3, int64_t offset, int64_t window, int64_t sinks, float scale,
                     void *stream) {
-  TTB_CHECK(q && k && v && out, "null tensor");
+  TTB_CHECK((seq_q == 0 || (q && out)) && (seq_q == 0 || seq_kv == 0 || (k && v)), "null tensor"); // an empty tensor may have no address
   TTB_CHECK(batch > 0 && heads_q > 0 && heads_kv > 0 && seq_q >= 0 && seq_kv >= 0 && head_dim > 0, "bad extents");
   TTB_CHECK(heads_q % heads_kv == 0, "query heads must be a multiple of kv heads");
   TTB_CHECK(batch <= 65535 && heads_kv <= 65535 && heads_q <= 1 << 20, "batch and kv heads are limited to 65535");
