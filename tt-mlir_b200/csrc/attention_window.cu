@@ -782,6 +782,7 @@ int ttb_sdpa_window(const void *q, const void *k, const void *v, const void *kv_
     setLastError("sdpa_window: head_dim is limited to 256");
     return TTB_ERR_UNSUPPORTED;
   }
+  TTB_CHECK(alignedTo(es, q, k, v, out) && alignedTo(4, kv_lens), "tensors must be aligned to their elements");
   if (seq_q == 0) return TTB_OK;
   const int64_t qd[3] = {heads_q * seq_q * head_dim, seq_q * head_dim, head_dim}, kd[3] = {heads_kv * seq_kv * head_dim, seq_kv * head_dim, head_dim};
   const int64_t *qs = q_strides3 ? q_strides3 : qd, *ks = k_strides3 ? k_strides3 : kd, *vs = v_strides3 ? v_strides3 : kd,
@@ -833,6 +834,7 @@ int ttb_sdpa_window_decode(const void *q, const void *k, const void *v, const vo
   if (rc) return rc;
   TTB_CHECK(window >= 1, "window must be positive");
   TTB_CHECK(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(workspace), "tensors must be 16-byte aligned");
+  TTB_CHECK(alignedTo(4, page_table, cur_pos), "tensors must be aligned to their elements");
   const int64_t positions = static_cast<int64_t>(pages_per_user) * block_size;
   WindowParams p;
   windowCommon(p, batch, 1, heads, kv_heads, positions, window, sinks, scale);
@@ -874,6 +876,7 @@ int ttb_sdpa_tree(const void *q, const void *k_draft, const void *v_draft, const
   TTB_CHECK(static_cast<int64_t>(nodes) * (heads / kv_heads) <= 1 << 24, "too many query rows per kv head");
   TTB_CHECK(aligned16(q) && aligned16(k_draft) && aligned16(v_draft) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) &&
                 aligned16(workspace), "tensors must be 16-byte aligned");
+  TTB_CHECK(alignedTo(4, page_table, cached_lens, parents, draft_lens), "tensors must be aligned to their elements");
   const int64_t positions = static_cast<int64_t>(pages_per_user) * block_size;
   WindowParams p;
   windowCommon(p, batch, nodes, heads, kv_heads, positions, window, sinks, scale);

@@ -214,6 +214,7 @@ int ttb_paged_commit_draft(void *const *host_caches, const void *const *host_dra
   TTB_CHECK(heads * head_dim * es <= 0x7fffffff, "a token's row is limited to 2^31 bytes");
   if (n_caches == 0 || users == 0 || nodes == 0) return TTB_OK;
   TTB_CHECK(host_caches && host_drafts && page_table && cached_lens && path && path_lens, "null tensor");
+  TTB_CHECK(alignedTo(4, page_table, cached_lens, path, path_lens), "tensors must be aligned to their elements");
   for (int i = 0; i < n_caches; ++i) TTB_CHECK(host_caches[i] && host_drafts[i], "null cache or draft");
   const int unit = unitOf(head_dim * es, host_caches, host_drafts, n_caches);
   const int rowUnits = static_cast<int>(head_dim * es / unit);

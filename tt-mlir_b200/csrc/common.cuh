@@ -193,6 +193,8 @@ __device__ __forceinline__ void st16(T *p, const Vec16<T> &r) {
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// All pointers (null ones too) are multiples of an element's size, a power of two: what a kernel loads elements through.
+template <typename... P> inline bool alignedTo(size_t size, const P *...p) { return ((reinterpret_cast<uintptr_t>(p) | ... | 0) & (size - 1)) == 0; }
 
 // Dispatch a callable templated on the C++ element type of a dtype tag.
 #define TTB_DISPATCH_DTYPE(dt, T, ...)                                                   \

@@ -1083,10 +1083,13 @@ int ttb_sample_logits(const void *logits, const void *uniform, const void *tempe
   TTB_CHECK(row_stride >= vocab || rows <= 1, "rows overlap");
   if (rows == 0) return TTB_OK;
   TTB_CHECK(logits && uniform && out, "null tensor");
+  const size_t es = dtypeSize(dtype);
+  TTB_CHECK((es == 0 || alignedTo(es, logits)) && alignedTo(4, uniform, temperature, top_k, top_p, min_p, out, prob),
+            "tensors must be aligned to their elements");
   (void)workspace;
   (void)workspace_bytes;
   cudaStream_t st = asStream(stream);
-  ProfScope prof("sample_logits", 4.0 * double(rows) * vocab, double(rows) * vocab * dtypeSize(dtype), st);
+  ProfScope prof("sample_logits", 4.0 * double(rows) * vocab, double(rows) * vocab * es, st);
   TTB_DISPATCH_FLOAT(dtype, T, return launchSample<T>(logits, uniform, temperature, top_k, top_p, min_p, out, prob, rows, vocab, row_stride, st))
   return TTB_OK;
 }
