@@ -114,6 +114,29 @@ def test_a_prompt_without_keys_is_zero(kn, dtype, D):
     assert (kn.download(out, q.shape, dtype) == 0).all()
 
 
+# ---- long prompts, far positions ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,H,Hkv,S,N,D,offset,window,sinks,lens", [
+    (torch.bfloat16, 4, 1, 1100, 4700, 128, 3600, 2900, 70, None),          # some 47 key tiles: the ring turns many times
+    (torch.float16, 2, 2, 900, 5000, 64, 4100, 10 ** 9, 0, None),
+    (torch.bfloat16, 3, 1, 700, 4000, 128, 3300, 3100, 1, [3777]),
+    (torch.float16, 4, 2, 300, 3000, 256, 2700, 2000, 5, None),
+    (torch.bfloat16, 4, 2, 140, 90, 128, 2 ** 29, 300, 3, None),            # the last positions there are: only the sinks are near
+    (torch.float16, 4, 2, 140, 90, 64, 2 ** 29, 2 ** 31, 0, [77]),          # ... or everything is
+    (torch.bfloat16, 2, 1, 70, 90, 32, 2 ** 29, 64, 80, None),
+    (torch.float32, 2, 1, 70, 90, 64, 2 ** 29, 2 ** 40, 80, None)])
+def test_long_and_far_prompts(kn, dtype, H, Hkv, S, N, D, offset, window, sinks, lens):
+    gen = torch.Generator().manual_seed(N + S)
+    q, k, v = rand(gen, 1, H, S, D, dtype=dtype), rand(gen, 1, Hkv, N, D, dtype=dtype), rand(gen, 1, Hkv, N, D, dtype=dtype)
+    seen = window_seen(torch.arange(S) + offset, N, window, sinks)
+    if lens:
+        seen[:, lens[0]:] = False
+    dead = ~seen.any(dim=0)
+    k[0][:, dead], v[0][:, dead] = NAN, float("inf")
+    got = kn.window(q, k, v, offset, window, sinks, torch.tensor(lens, dtype=torch.int32) if lens else None)
+    want, tol = attend(q[0], k[0], v[0], seen, 1 / math.sqrt(D), dtype)
+    check(got[0], want, tol)
+
+
 # ---- scales and parents in long caches -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("scale", [0.0, -0.5])
 @pytest.mark.parametrize("B,H,Hkv,D,room", [(1, 4, 1, 64, 4352), (5, 16, 8, 128, 4352), (18, 8, 8, 64, 4352), (2, 8, 2, 128, 300)])
