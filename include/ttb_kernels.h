@@ -473,7 +473,7 @@ TTB_API int ttb_sampling(const void *values, const void *indices, const void *k,
  * logits are never taken; a row of nothing else gives -1 and 0.  A weight below 2^-60 of the row's largest may count as
  * none.  Weights and their sums hold to 2^-36 of themselves: the token is the definition's unless uniform or top_p lies that
  * near to a border.  vocab is limited to 2^22.  The same inputs give the same token on every run.
- * `workspace`: ttb_sample_logits_workspace_bytes(...), not shared by calls that can overlap on the GPU.
+ * No workspace is needed: ttb_sample_logits_workspace_bytes(...) is 0, and `workspace` may be null.
  * ttb_sampling draws among pre-selected candidates with its own generator (operations/reduction/sampling.cpp). */
 TTB_API size_t ttb_sample_logits_workspace_bytes(int64_t rows, int64_t vocab);
 TTB_API int ttb_sample_logits(const void *logits, const void *uniform, const void *temperature, const void *top_k, const void *top_p,

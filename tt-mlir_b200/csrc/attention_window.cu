@@ -20,7 +20,7 @@
 // With few users the slots are split over `splits` CTAs: up to 8 are a cluster and join their parts through its shared
 // memory, parts of more go through the workspace and a second kernel.
 // Measured: one token for each of 64 users, 32 query / 8 kv heads x 128, window 4096, 16 sinks, bf16: 192 us, 85 % of the
-// measured HBM rate; one user, 8 heads x 64, window 1000: 10 us, of which a launch that does nothing takes 8.
+// measured HBM rate; one user, 8 heads x 64, window 1000: 10 us a call from Python, 6 replayed from a graph.
 #include "attention_cached.cuh"
 #include "common.cuh"
 
@@ -515,7 +515,9 @@ __global__ void __launch_bounds__(128) windowJoinKernel(T *__restrict__ out, Win
 }
 
 // The general form for prompts: any float type, any head_dim up to 256, any strides (head_dim contiguous).  One warp
-// per query row; 32 keys at a time, each lane the dot product of one key, then the lanes share the value columns.
+// per query row; 32 keys at a time, each lane the dot product of one key, then the lanes share the value columns.  Nothing is
+// shared between rows and neighbouring lanes read whole keys apart: 32 / 8 heads x 128, f32, 2048 tokens, window 512 take 14.7
+// ms (1 TFLOP/s).
 template <typename T>
 __global__ void __launch_bounds__(128)
     windowRowKernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ out, WindowParams p, int D) {
@@ -603,7 +605,10 @@ static TreePlan treePlan(int64_t batch, int64_t nodes, int64_t heads, int64_t kv
   // The tensor-core kernel reads faster but starts slower (128 KB of ring to fill, tensor memory to claim, a second kernel
   // for the join).  Measured with 8 kv heads x 4, head_dim 128, this kernel / that one, us: 1 user, 2500 tokens, 8 nodes
   // 29 / 21, 4000 tokens, 8 .. 32 nodes 30 .. 36 / 23 .. 35, 7000 tokens 35 / 40; 4 users, 4000 tokens, 8 nodes 36 / 30; 16
-  // users, 2500 tokens, 8 nodes 49 / 61, 8192 tokens, 4 nodes 107 / 120, 16 nodes 109 / 177.
+  // users, 2500 tokens, 8 nodes 49 / 61, 8192 tokens, 4 nodes 107 / 120, 16 nodes 109 / 177.  Replayed from a graph, 1 kv head
+  // x 8, head_dim 128, 8 nodes, the other kernel / this one: 1 user, 4000 tokens 23 / 23, 7000 tokens 32 / 29, 8 users, 7000
+  // tokens 34 / 29.  With head_dim 64 the rule comes too early: 8 kv heads x 4, 8 nodes, 1 user, 7000 tokens 19 / 25, 16000
+  // tokens 35 / 32, 8 users, 7000 tokens 35 / 45, 40 users, 2500 tokens 56 / 80.
   t.tall = (dim == 64 || dim == 128) && (slots > 4096 || (slots >= 2048 && 2 * batch * kvHeads > smCount()));
   if (!t.tall) {
     t.splits = windowSplits(batch, kvHeads, rows, slots);

@@ -3,8 +3,9 @@
 //                          beams are reordered, live blocks move into holes before the pool shrinks
 //  ttb_paged_commit_draft  the accepted path of a verified draft tree is appended to its user's cached sequence
 // Both only move bytes: the bound is HBM (each byte read and written once), or the launch when there is little to move.
-// Measured: 96 blocks of 64 KB in 32 caches 55.6 us (7.3 TB/s, the sources partly from L2), one block in 2 caches 8.6; the
-// paths of 48 users (up to 31 rows of 2 KB) in 32 caches 21.4 us (4.6 TB/s; 29.6 with the places looked up per cache).
+// Measured: 96 blocks of 64 KB in 32 caches 55.6 us (6.3 TB/s: the 96 have some 72 sources), one block in 2 caches 8.6 (1.6 of
+// it on the GPU); the paths of 48 users (up to 31 rows of 2 KB) in 32 caches 20.2 us (4.8 TB/s; 29.6 with the places looked
+// up per cache).
 #include "common.cuh"
 
 #include <algorithm>
