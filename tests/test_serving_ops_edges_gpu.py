@@ -291,6 +291,31 @@ def test_sample_keeps_the_prefix_next_to_a_border(kn, dtype, k):
     assert ((prob.double() - shares).abs() <= 2.0 ** -23 * shares).all()
 
 
+@pytest.mark.parametrize("vocab", [9000, 60000])
+def test_sample_rows_whose_tops_a_sample_misses(kn, vocab):
+    """A few logits far above all others, by 20 to 1500 nats, the next ones 5 and 9 nats below: what top-p and top-k keep is
+    among them, whatever the reference that the first pass took its weights against."""
+    gen = torch.Generator().manual_seed(74)
+    rise = [20, 60, 150, 204, 206, 215, 250, 270, 280, 300, 400, 500, 600, 620, 640, 700, 1000, 1500]
+    rows = 4 * len(rise)
+    logits = torch.randn(rows, vocab, generator=gen)
+    for r in range(rows):
+        at = torch.randperm(vocab, generator=gen)[:4]
+        logits[r, at] = rise[r // 4] + torch.tensor([0.0, -5.0, -9.0, -9.0])
+    p = [0.9, 0.999, 0.9999, 1.0] * len(rise)
+    k = [0, 0, 3, 0] * len(rise)
+    token, prob = kn.sample(logits, torch.rand(rows, generator=gen), None, torch.tensor(k, dtype=torch.int32), torch.tensor(p))
+    for r in range(rows):
+        x = logits[r].double()
+        kept = torch.sort(x, descending=True, stable=True).indices[:k[r] or vocab]
+        w = torch.exp(x[kept] - x[kept[0]])
+        limit = float(torch.tensor(p[r], dtype=torch.float32))
+        kept = kept[(torch.cumsum(w, 0) - w) < limit * w.sum()] if p[r] < 1 else kept
+        w = torch.exp(x[kept] - x[kept[0]])
+        share = float(w[kept == int(token[r])].sum() / w.sum())
+        assert share > 0 and abs(float(prob[r]) - share) <= 2.0 ** -23 * share, (r, float(prob[r]), share)
+
+
 def test_sample_min_p_at_its_border(kn):
     """min-p is the weight of one token, rounded down or up to f32: the token stays or goes.  Under a very high temperature
     every finite logit weighs 1, which min-p 1 keeps."""

@@ -45,7 +45,7 @@ constexpr float SL_FLOOR = 60.0f;           // octaves below the largest weight 
 constexpr int SL_UNITS = 36;                // a list's largest weight is at most 2^36 units
 constexpr int SL_HALF = 18;                 // ... in two halves, which are summed as unsigned 32-bit numbers
 constexpr int SL_SIDE = 4;                  // weights computed side by side
-constexpr double SL_RISE = 900.0;           // octaves that a logit may lie above the reference
+constexpr double SL_RISE = 300.0;           // octaves that a logit may lie above the reference, within the 400 that weights reach down to
 constexpr int64_t SL_MAX_VOCAB = 1 << 22;
 static_assert(SL_BINS == 2 * SL_THREADS, "bins per thread");
 static_assert(int64_t(SL_THREADS) * SL_KEEP << SL_HALF < int64_t(1) << 32 && SL_UNITS == 2 * SL_HALF, "the halves' sums fit unsigned 32 bits");
