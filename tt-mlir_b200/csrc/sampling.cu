@@ -20,7 +20,7 @@
 //  * The draw is a search too: of the warps' runs the one that holds u times the total is split among the warps
 //    again, until there is a thread for each entry.  After a cut the last pass knows the runs' weights already.
 // Measured, 256 rows of 128000 f32 logits (131 MB, 20 us at HBM speed), us: largest logit 48, no cut 72, top-k 50 70, top-k
-// 50 and top-p 0.9 128, top-k 40000 180, top-p 0.99 (flat rows) 257, everything mixed 230.  With weights of f32 exponentials
+// 50 and top-p 0.9 127, top-k 40000 178, top-p 0.99 (flat rows) 250 to 280, everything mixed 230.  With weights of f32 exponentials
 // it was 43, 41, 62, 79, 103, 166 and 141, and the tokens were not the definition's (see Weigher).  What bounds it: a pass
 // that weighs issues some 35 to 40 instructions per entry, 14 of them f64, and takes some 110 thousand of a row's clocks with
 // two rows per SM (one that only compares 50; their reads 38 at HBM speed); the steps between passes, which depend on one
@@ -44,7 +44,7 @@ constexpr float SL_FIRST = 2500.0f;         // entries aimed at by the first pas
 constexpr float SL_FLOOR = 60.0f;           // octaves below the largest weight that count
 constexpr int SL_UNITS = 36;                // a list's largest weight is at most 2^36 units
 constexpr int SL_HALF = 18;                 // ... in two halves, which are summed as unsigned 32-bit numbers
-constexpr int SL_SIDE = 4;                  // weights computed side by side
+constexpr int SL_SIDE = 4;                  // weights computed side by side (2, 4, 8 of them: 290, 245, 286 us with mixed settings)
 constexpr double SL_RISE = 300.0;           // octaves that a logit may lie above the reference, within the 400 that weights reach down to
 constexpr int64_t SL_MAX_VOCAB = 1 << 22;
 static_assert(SL_BINS == 2 * SL_THREADS, "bins per thread");
@@ -839,7 +839,8 @@ __global__ void __launch_bounds__(SL_THREADS, 2)
       int which = cutK ? 0 : 1, round = 0;
       for (bool done = false; !done;) {
         if (ask) {
-          // The first interval is open unless top-k is too deep for that (top-k 40000: 154 us with an open one, 108 closed, with weights in f32).
+          // The first interval is open unless top-k is too deep for that (256 rows of 128000, top-k 40000: 195 us with an open one, 178 closed;
+          // mixed settings 300 and 239).
           slChoose(s, weigh.octaves(), below, above, sLeast, top, byMass, first ? !cutK || want <= 0.6f * SL_FIRST : up, want, have, n, samples);
           float nLo = s->lo, nHi = s->hi;
           if (first) {
